@@ -359,6 +359,62 @@ int cs_dice_ce_backward(const float* logits, const int64_t* logit_strides, const
                         const void* workspace, size_t workspace_bytes, float* grad_logits, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Losses of a linear head over a large vocabulary (no counterpart in the reference, whose loss has 3 classes).  z = hidden weight^T is
+ * never held whole: the forward pass keeps per row its maximum and sum, the backward pass rebuilds z in pieces of the vocabulary.
+ *   CS_HEAD_CROSS_ENTROPY  loss_i = lse(z_i) - z_i[target_i];  a row whose target is ignore_index has loss 0 and is not counted
+ *   CS_HEAD_DISTILLATION   q_i = softmax(teacher_i / T) over the row's `top` entries, loss_i = T^2 sum_k q_ik (log q_ik - log p_i[id_ik]),
+ *                          p_i = softmax(z_i / T) over the whole vocabulary.  An entry with a negative id or a teacher logit of -inf
+ *                          carries no mass; a row without mass has loss 0 and is not counted.  An id may come twice in a row.
+ * reduction CS_REDUCE_MEAN divides the sum by the number of counted rows (no counted row: 0), in 64 bits and in a fixed order.
+ * A target or id >= vocab (or a negative target other than ignore_index) makes the row's loss and gradients NaN.
+ * hidden [rows][width] and weight [vocab][width] have `type`, unit inner stride and the given pitch in elements; rows whose start, pitch
+ * or length is not a multiple of 16 bytes are first copied into the workspace.  Sums, maxima and losses are held in 32 bits or more.
+ * The backward pass needs the same descriptor, the `saved` bytes of its forward pass, and `grad` = d / d loss (device float; for
+ * CS_REDUCE_NONE one per row, grad_stride floats apart); either gradient may be NULL.  Results do not depend on the launch order (no
+ * atomics).  Gradients are contiguous and start at a multiple of 16 bytes.  Limits: 1 <= width < 2^21, 1 <= vocab < 2^30, 0 <= rows < 2^26, 1 <= top <= 1024, finite temperature > 0.
+ * ---------------------------------------------------------------------------------------------- */
+enum { CS_TYPE_BF16 = 0, CS_TYPE_FP16 = 1, CS_TYPE_FP32 = 2 };
+enum { CS_HEAD_CROSS_ENTROPY = 0, CS_HEAD_DISTILLATION = 1 };
+enum { CS_REDUCE_NONE = 0, CS_REDUCE_MEAN = 1, CS_REDUCE_SUM = 2 };
+typedef struct cs_head_loss {
+    const void* hidden;
+    const void* weight;
+    const void* ids;            /* cross entropy: target [rows]; distillation: [rows][top] */
+    const void* teacher;        /* distillation: logits [rows][top]; else NULL */
+    int64_t hidden_pitch, weight_pitch, ids_pitch, teacher_pitch;   /* elements between rows */
+    int64_t rows, vocab, width;
+    int64_t ignore_index;
+    double temperature;         /* distillation; the cross entropy takes 1 */
+    int type, kind, reduction;
+    int ids_bits;               /* 32 or 64 */
+    int teacher_type;           /* CS_TYPE_* */
+    int top;                    /* distillation; the cross entropy takes 1 */
+} cs_head_loss;
+size_t cs_head_loss_saved_bytes(const cs_head_loss* head_host);
+/* backward: 0 the forward pass; else the backward pass with the gradients wanted (bit 0: hidden, bit 1: weight) */
+size_t cs_head_loss_workspace_bytes(const cs_head_loss* head_host, int backward);
+/* row_losses: [rows] or NULL; loss: the reduced loss or NULL (CS_REDUCE_NONE) */
+int cs_head_loss_forward(const cs_head_loss* head_host, float* row_losses, float* loss, void* saved, size_t saved_bytes, void* workspace,
+                         size_t workspace_bytes, void* stream);
+int cs_head_loss_backward(const cs_head_loss* head_host, const void* saved, size_t saved_bytes, const float* grad, int64_t grad_stride,
+                          void* grad_hidden, void* grad_weight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Microscaled 4-bit numbers (OCP MX, MXFP4; no counterpart in the reference).  32 values along the inner axis share an e8m0 scale
+ * 2^(s - 127), s = floor(log2 max|x|) + 125 clamped at 0; a value is x / scale rounded to e2m1 (ties to even, above 6 to 6).
+ * codes [rows][16 * blocks] (two a byte, the even one low), scales [rows][blocks], blocks = ceil(width / 32); a last block is filled up
+ * with zeros.  A block that holds an infinity or a NaN has the scale 255, which reads as NaN.  x: `pitch` elements between rows, unit
+ * inner stride.  cs_mxfp4_linear quantises x and multiplies it with quantised weights, y[r][o] = sum_k x[r][k] w[o][k] with fp32 sums
+ * and one rounding to `type` (CS_TYPE_*, of x and y); y is contiguous.  No gradients.
+ * Limits: 0 <= rows, outputs < 2^30, 1 <= width < 2^24; codes (linear: and y) start at a multiple of 4 (linear: 16) bytes.
+ * ---------------------------------------------------------------------------------------------- */
+int cs_mxfp4_quantize(const void* x, int64_t pitch, int64_t rows, int64_t width, int type, uint8_t* codes, uint8_t* scales, void* stream);
+int cs_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t width, int type, void* out, void* stream);
+size_t cs_mxfp4_linear_workspace_bytes(int64_t rows, int64_t width, int64_t outputs);
+int cs_mxfp4_linear(const void* x, int64_t pitch, int64_t rows, int64_t width, int type, const uint8_t* codes, const uint8_t* scales, int64_t outputs,
+                    void* y, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Optimiser  -  replaces `optimizer = torch.optim.AdamW(model.parameters(), args.initial_lr)` ... `optimizer.step()`
  * (baseline/model_training_3class.py:237, :262) with torch's update rule (amsgrad / maximize off) for ALL tensors in one launch:
  *   p *= 1 - lr wd;  m += (g - m)(1 - b1);  v = b2 v + (1 - b2) g^2;  p -= lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)

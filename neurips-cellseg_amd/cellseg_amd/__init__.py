@@ -7,6 +7,9 @@ Host-side mirror of the reference's interfaces (same names, arguments and error 
   create_interior_map        <- data/pre_process_3class.py:31-56
   DiceCELoss / AdamW         <- monai.losses.DiceCELoss(softmax=True) / torch.optim.AdamW (baseline/model_training_3class.py:234-237)
   TrainStep                  <- the loop body baseline/model_training_3class.py:250-262 as one captured launch sequence (hipGraph)
+Beyond the reference, next to its loss and to the fp8 mode:
+  linear_cross_entropy, linear_distillation   losses of a linear head over a large vocabulary, without its logits in memory
+  mxfp4_quantize, mxfp4_linear                microscaled 4-bit numbers and the linear layer on them
 All arithmetic runs in libcellseg_hip.so; importing this package without the built library raises.
 """
 from ._lib import CellSegHipError, LIB_PATH, lib  # noqa: F401
@@ -15,9 +18,12 @@ from .inferers import (balanced_batch, make_plan, rank_rows, sliding_window_infe
                        window_starts)
 from .postprocess import StripLabeller, create_interior_map, label, mask_to_instances, mask_to_instances_strips, prob_to_instances  # noqa: F401
 from .losses import DiceCELoss, one_hot  # noqa: F401
+from .head_losses import LinearCrossEntropyLoss, LinearDistillationLoss, linear_cross_entropy, linear_distillation  # noqa: F401
+from .mxfp4 import MXFP4Tensor, mxfp4_linear, mxfp4_quantize  # noqa: F401
 from .optim import AdamW  # noqa: F401
 from .trainer import TrainStep  # noqa: F401
 from . import metrics, parallel  # noqa: F401
 
 __all__ = ["UNet", "sliding_window_inference", "swi_infer_image", "make_plan", "window_starts", "rank_rows", "strip_partition", "swi_infer_strip", "share_partition", "swi_infer_share",
-           "label", "mask_to_instances", "mask_to_instances_strips", "StripLabeller", "prob_to_instances", "create_interior_map", "DiceCELoss", "one_hot", "AdamW", "TrainStep", "CellSegHipError", "lib", "LIB_PATH"]
+           "label", "mask_to_instances", "mask_to_instances_strips", "StripLabeller", "prob_to_instances", "create_interior_map", "DiceCELoss", "one_hot", "linear_cross_entropy", "linear_distillation", "LinearCrossEntropyLoss", "LinearDistillationLoss",
+           "MXFP4Tensor", "mxfp4_quantize", "mxfp4_linear", "AdamW", "TrainStep", "CellSegHipError", "lib", "LIB_PATH"]

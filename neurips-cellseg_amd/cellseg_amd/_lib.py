@@ -35,6 +35,14 @@ class SwiShare(C.Structure):
         return [tuple(self.rect[i]) for i in range(self.n_rects)]
 
 
+class HeadLoss(C.Structure):
+    """Mirror of ``cs_head_loss``."""
+    _fields_ = ([(n, C.c_void_p) for n in ("hidden", "weight", "ids", "teacher")]
+                + [(n, C.c_int64) for n in ("hidden_pitch", "weight_pitch", "ids_pitch", "teacher_pitch", "rows", "vocab", "width", "ignore_index")]
+                + [("temperature", C.c_double)]
+                + [(n, C.c_int) for n in ("type", "kind", "reduction", "ids_bits", "teacher_type", "top")])
+
+
 class SwiPlan(C.Structure):
     """Mirror of ``cs_swi_plan``."""
     _fields_ = [(n, C.c_int) for n in ("img_h", "img_w", "roi_h", "roi_w", "pad_top", "pad_left", "pad_h", "pad_w",
@@ -110,6 +118,14 @@ def _load() -> C.CDLL:
                                      vp, vp, sz, vp]),
         "cs_dice_ce_backward": (i32, [vp, C.POINTER(i64), vp, C.POINTER(i64), i32, i32, i32, i32, C.c_float, C.c_float, C.c_float, C.c_float,
                                       vp, vp, sz, vp, vp]),
+        "cs_head_loss_saved_bytes": (sz, [C.POINTER(HeadLoss)]),
+        "cs_head_loss_workspace_bytes": (sz, [C.POINTER(HeadLoss), i32]),
+        "cs_head_loss_forward": (i32, [C.POINTER(HeadLoss), vp, vp, vp, sz, vp, sz, vp]),
+        "cs_head_loss_backward": (i32, [C.POINTER(HeadLoss), vp, sz, vp, i64, vp, vp, vp, sz, vp]),
+        "cs_mxfp4_quantize": (i32, [vp, i64, i64, i64, i32, vp, vp, vp]),
+        "cs_mxfp4_dequantize": (i32, [vp, vp, i64, i64, i32, vp, vp]),
+        "cs_mxfp4_linear_workspace_bytes": (sz, [i64, i64, i64]),
+        "cs_mxfp4_linear": (i32, [vp, i64, i64, i64, i32, vp, vp, i64, vp, vp, sz, vp]),
         "cs_adamw_step": (i32, [vp, i32, i64, vp, vp, vp, C.c_float, C.c_float, C.c_float, C.c_float, C.c_float, i32, vp]),
         "cs_unet_bind_params": (i32, [vp, C.POINTER(vp), i32, vp]),
         "cs_unet_repack": (i32, [vp, vp]),
@@ -140,6 +156,8 @@ EXPORTED = ("cs_last_error cs_version cs_device_count cs_unet_create cs_unet_des
             "cs_normalize_image cs_label_max cs_label_overlap cs_remove_boundary_workspace_bytes cs_remove_boundary_cells "
             "cs_augment_workspace_bytes cs_augment_batch cs_label_deflate_workspace_bytes cs_label_deflate_bound cs_label_deflate cs_ccl_workspace_bytes "
             "cs_ccl_postprocess cs_ccl_label cs_ccl_strip_halo cs_ccl_strip_edge_ints cs_ccl_seam_workspace_bytes cs_ccl_strip_local cs_ccl_strip_resolve cs_ccl_strip_finish cs_interior_map cs_dice_ce_workspace_bytes cs_dice_ce_forward cs_dice_ce_backward cs_adamw_step "
+            "cs_head_loss_saved_bytes cs_head_loss_workspace_bytes cs_head_loss_forward cs_head_loss_backward cs_mxfp4_quantize cs_mxfp4_dequantize "
+            "cs_mxfp4_linear_workspace_bytes cs_mxfp4_linear "
             "cs_unet_bind_params cs_unet_repack cs_unet_readback cs_adamw_step_dev cs_graph_begin cs_graph_end cs_graph_abort cs_graph_launch "
             "cs_graph_num_nodes cs_graph_destroy cs_prof_is_enabled cs_prof_enable cs_prof_reset cs_prof_collect").split()
 

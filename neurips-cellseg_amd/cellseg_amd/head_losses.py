@@ -1,0 +1,165 @@
+"""``linear_cross_entropy`` / ``linear_distillation`` - the losses of a linear head over a large vocabulary, next to ``DiceCELoss``.
+
+The logits ``hidden @ weight.T`` are never held: the forward pass keeps the maximum and the sum of exponentials of every row, the backward
+pass rebuilds the logits in pieces of the vocabulary (``cs_head_loss_forward`` / ``cs_head_loss_backward``, csrc/kernels_head.hip).
+With rows i, vocabulary j, ``z = hidden weight^T``, ``p_i = softmax(z_i / T)``:
+
+    cross entropy   loss_i = -log p_i[target_i]                                       T = 1
+    distillation    loss_i = T^2 sum_k q_ik (log q_ik - log p_i[teacher_ids_ik])      q_i = softmax(teacher_logits_i / T)
+
+``hidden`` ``[..., D]`` and ``weight`` ``[V, D]`` share one type (bfloat16, float16 or float32) and get gradients of that type; products are
+summed, and losses returned, in float32.  16-bit gradients of the logits are rounded once to the type of the inputs before they are
+multiplied.  A float16 net wants the usual loss scale: a mean over many rows makes gradients smaller than float16 holds.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+import torch.nn as nn
+
+from . import _lib
+from ._lib import check, lib
+
+TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}          # CS_TYPE_*
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}                            # CS_REDUCE_*
+_CROSS_ENTROPY, _DISTILLATION = 0, 1
+MAX_TOP = 1024
+
+
+def _pitch(t: torch.Tensor) -> int:
+    """Elements between the rows of a 2-d tensor with unit inner stride (of one row: its length)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def rows_of(t: torch.Tensor) -> torch.Tensor:
+    """[..., D] -> [rows, D] with unit inner stride and rows that do not overlap; a copy only where the strides do not allow a view."""
+    t = t.reshape(-1, t.shape[-1])
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t
+
+
+def _checked(hidden: torch.Tensor, weight: torch.Tensor, reduction: str, ids: torch.Tensor, name: str):
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction is one of {', '.join(_REDUCTIONS)}, got {reduction!r}")
+    if hidden.dtype not in TYPES or weight.dtype != hidden.dtype:
+        raise TypeError(f"hidden and weight share one of bfloat16, float16 and float32, got {hidden.dtype} and {weight.dtype}")
+    if hidden.dim() < 1 or weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"expected hidden [..., D] and weight [V, D], got {tuple(hidden.shape)} and {tuple(weight.shape)}")
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"{name} holds int64 or int32, got {ids.dtype}")
+    for t in (hidden, weight, ids):
+        _lib.require_gpu(t)
+        if t.device != hidden.device:
+            raise ValueError(f"hidden, weight and {name} are on one device, got {hidden.device} and {t.device}")
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *, ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+    """Softmax cross entropy of the logits ``hidden @ weight.T`` against ``target`` (``hidden.shape[:-1]``, int64 or int32) -> float32.
+
+    Rows whose target is ``ignore_index`` have loss 0, no gradient, and are not counted; a mean over no row is 0.  Any other target
+    outside ``[0, V)`` makes the loss and the gradients NaN (it is seen on the device only)."""
+    _checked(hidden, weight, reduction, target, "target")
+    if target.shape != hidden.shape[:-1]:
+        raise ValueError(f"expected target {tuple(hidden.shape[:-1])}, got {tuple(target.shape)}")
+    losses = _HeadLoss.apply(rows_of(hidden), rows_of(weight), target.reshape(-1), None, _CROSS_ENTROPY, _REDUCTIONS[reduction], int(ignore_index), 1.0)
+    return losses.reshape(target.shape) if reduction == "none" else losses
+
+
+def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *, temperature: float = 1.0,
+                        reduction: str = "mean") -> torch.Tensor:
+    """T^2 KL(teacher || student) of the student logits ``hidden @ weight.T`` against a teacher's top logits -> float32.
+
+    ``teacher_ids`` (int64 or int32) and ``teacher_logits`` (bfloat16, float16 or float32) are ``[..., K]``, K up to 1024, in any order; the
+    teacher's mass is spread over them alone, the student's over the whole vocabulary.  An entry with a negative id or a logit of -inf
+    carries no mass; rows without mass have loss 0, no gradient, and are not counted; an id may come twice.  An id >= V makes the loss
+    and the gradients NaN.  The teacher gets no gradient."""
+    _checked(hidden, weight, reduction, teacher_ids, "teacher_ids")
+    if teacher_ids.dim() != hidden.dim() or teacher_ids.shape[:-1] != hidden.shape[:-1] or teacher_logits.shape != teacher_ids.shape:
+        raise ValueError(f"expected teacher_ids and teacher_logits {tuple(hidden.shape[:-1])} + (K,), got {tuple(teacher_ids.shape)} and {tuple(teacher_logits.shape)}")
+    if not 1 <= teacher_ids.shape[-1] <= MAX_TOP:
+        raise ValueError(f"a teacher gives 1 to {MAX_TOP} logits per row, got {teacher_ids.shape[-1]}")
+    if teacher_logits.dtype not in TYPES:
+        raise TypeError(f"teacher_logits holds bfloat16, float16 or float32, got {teacher_logits.dtype}")
+    if teacher_logits.device != hidden.device:
+        raise ValueError(f"teacher_logits is on {teacher_logits.device}, hidden on {hidden.device}")
+    if teacher_logits.requires_grad and torch.is_grad_enabled():
+        raise ValueError("the teacher gets no gradient: pass teacher_logits.detach()")
+    if not 0.0 < float(temperature) < 1e30:
+        raise ValueError(f"temperature is positive and finite, got {temperature}")
+    losses = _HeadLoss.apply(rows_of(hidden), rows_of(weight), rows_of(teacher_ids), rows_of(teacher_logits), _DISTILLATION, _REDUCTIONS[reduction], 0, float(temperature))
+    return losses.reshape(hidden.shape[:-1]) if reduction == "none" else losses
+
+
+class LinearCrossEntropyLoss(nn.Module):
+    """``linear_cross_entropy`` as a module: ``loss(hidden, weight, target)``."""
+
+    def __init__(self, ignore_index: int = -100, reduction: str = "mean"):
+        super().__init__()
+        if reduction not in _REDUCTIONS:
+            raise ValueError(f"reduction is one of {', '.join(_REDUCTIONS)}, got {reduction!r}")
+        self.ignore_index, self.reduction = ignore_index, reduction
+
+    def forward(self, hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor) -> torch.Tensor:
+        return linear_cross_entropy(hidden, weight, target, ignore_index=self.ignore_index, reduction=self.reduction)
+
+
+class LinearDistillationLoss(nn.Module):
+    """``linear_distillation`` as a module: ``loss(hidden, weight, teacher_ids, teacher_logits)``."""
+
+    def __init__(self, temperature: float = 1.0, reduction: str = "mean"):
+        super().__init__()
+        if reduction not in _REDUCTIONS:
+            raise ValueError(f"reduction is one of {', '.join(_REDUCTIONS)}, got {reduction!r}")
+        if not 0.0 < float(temperature) < 1e30:
+            raise ValueError(f"temperature is positive and finite, got {temperature}")
+        self.temperature, self.reduction = temperature, reduction
+
+    def forward(self, hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor) -> torch.Tensor:
+        return linear_distillation(hidden, weight, teacher_ids, teacher_logits, temperature=self.temperature, reduction=self.reduction)
+
+
+def _descriptor(hidden, weight, kind, reduction, ignore_index, temperature, top, ids=None, teacher=None) -> _lib.HeadLoss:
+    return _lib.HeadLoss(hidden=hidden.data_ptr(), weight=weight.data_ptr(), ids=ids.data_ptr() if ids is not None else None,
+                         teacher=teacher.data_ptr() if teacher is not None else None, hidden_pitch=_pitch(hidden), weight_pitch=_pitch(weight),
+                         ids_pitch=(ids.stride(0) if ids.shape[0] > 1 else top) if ids is not None else 0, teacher_pitch=_pitch(teacher) if teacher is not None else 0,
+                         rows=hidden.shape[0], vocab=weight.shape[0], width=weight.shape[1], ignore_index=ignore_index, temperature=temperature,
+                         type=TYPES[hidden.dtype], kind=kind, reduction=reduction, ids_bits=32 if ids is not None and ids.dtype == torch.int32 else 64,
+                         teacher_type=TYPES[teacher.dtype] if teacher is not None else 0, top=top)
+
+
+class _HeadLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, ids, teacher, kind, reduction, ignore_index, temperature):
+        top = 1 if teacher is None else ids.shape[1]
+        head = _descriptor(hidden, weight, kind, reduction, ignore_index, temperature, top, ids, teacher)
+        with torch.cuda.device(hidden.device):
+            size = int(lib.cs_head_loss_saved_bytes(C.byref(head)))
+            if not size:
+                check(-1, "cs_head_loss_saved_bytes")
+            saved = torch.empty(size, dtype=torch.uint8, device=hidden.device)
+            ws = torch.empty(max(1, int(lib.cs_head_loss_workspace_bytes(C.byref(head), 0))), dtype=torch.uint8, device=hidden.device)
+            loss = torch.empty((hidden.shape[0],) if reduction == 0 else (), dtype=torch.float32, device=hidden.device)
+            to = C.c_void_p(loss.data_ptr())
+            check(lib.cs_head_loss_forward(C.byref(head), to if reduction == 0 else None, None if reduction == 0 else to, C.c_void_p(saved.data_ptr()), saved.numel(),
+                                           C.c_void_p(ws.data_ptr()), ws.numel(), _lib.stream_ptr()), "cs_head_loss_forward")
+        ctx.save_for_backward(hidden, weight, saved)
+        ctx.cfg = (kind, reduction, ignore_index, temperature, top)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        hidden, weight, saved = ctx.saved_tensors
+        head = _descriptor(hidden, weight, *ctx.cfg)
+        want = (1 if ctx.needs_input_grad[0] else 0) | (2 if ctx.needs_input_grad[1] else 0)
+        grad = grad.float()
+        with torch.cuda.device(hidden.device):
+            ws = torch.empty(max(1, int(lib.cs_head_loss_workspace_bytes(C.byref(head), want))), dtype=torch.uint8, device=hidden.device)
+            gh = torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device) if want & 1 else None
+            gw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if want & 2 else None
+            check(lib.cs_head_loss_backward(C.byref(head), C.c_void_p(saved.data_ptr()), saved.numel(), C.c_void_p(grad.data_ptr()), grad.stride(0) if grad.dim() else 0,
+                                            C.c_void_p(gh.data_ptr()) if want & 1 else None, C.c_void_p(gw.data_ptr()) if want & 2 else None,
+                                            C.c_void_p(ws.data_ptr()), ws.numel(), _lib.stream_ptr()), "cs_head_loss_backward")
+        return gh, gw, None, None, None, None, None, None

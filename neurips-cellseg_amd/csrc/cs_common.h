@@ -36,6 +36,7 @@ enum KernelId {
     K_WGRAD, K_TOP_BWD, K_PRE, K_METRIC, K_UNPACK, K_CONV3_WINO, K_LOSS, K_CONV3_WINO4, K_LABEL_DEFLATE,
     K_CONV3_S1_FP8, K_CONV3_S2_FP8, K_CONV1_FP8, K_CONVT_FP8,      // the e4m3 launches of the fp8 mode (their own matrix peak)
     K_CCL_SEAM,                                                    // edge records + seam union-find of the strip-local labelling
+    K_HEAD_LOSS, K_MXFP4,                                          // large-vocabulary head losses; 4-bit quantisation and linear layer
     K_NUM_IDS
 };
 const char* kernel_name(int id);

@@ -34,7 +34,8 @@ static const char* kNames[K_NUM_IDS] = {
     "conv_last_valu", "norm_finalize", "norm_act_add", "swi_finalize", "pack_weights", "ccl_init", "ccl_merge",
     "ccl_compress", "ccl_sizes", "ccl_filter", "ccl_count", "ccl_scan", "ccl_rank", "ccl_relabel", "memset", "norm_bwd",
     "colsum", "wgrad_mfma", "top_bwd_valu", "normalize_input", "f1_metric", "wgrad_unpack", "conv3x3_s1_wino", "dice_ce_loss", "conv3x3_s1_wino4",
-    "label_deflate", "conv3x3_s1_fp8", "conv3x3_s2_fp8", "conv1x1_fp8", "convT3x3s2_fp8", "ccl_seam"};
+    "label_deflate", "conv3x3_s1_fp8", "conv3x3_s2_fp8", "conv1x1_fp8", "convT3x3s2_fp8", "ccl_seam",
+    "head_loss", "mxfp4"};
 static_assert(K_NUM_IDS <= CS_PROF_MAX_KERNELS, "cs_prof_collect: the caller's arrays hold CS_PROF_MAX_KERNELS entries");
 const char* kernel_name(int id) { return (id >= 0 && id < K_NUM_IDS) ? kNames[id] : "?"; }
 

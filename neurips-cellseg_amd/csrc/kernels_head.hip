@@ -1,0 +1,816 @@
+// gfx950 (MI355X): losses of a linear head over a large vocabulary, without its logits in memory - the cross entropy and the
+// distillation from a teacher's top logits.  Both are one computation: row i has a sparse target distribution q_i over a few ids (the
+// cross entropy: one id, q = 1) and, with u = z / T, z = H W^T, lse_i = log sum_j exp(u_ij), p = exp(u - lse):
+//   loss_i = T^2 (sum_k q_ik log q_ik + lse_i - sum_k q_ik u_i[id_ik]),   d loss_i / d z = T (p_i - q_i)
+// Forward: one matrix product whose epilogue leaves, per row and tile of the vocabulary, the maximum and the sum of exponentials, and the
+// few z that the loss names; a wave per row joins them.  Backward, in pieces of the vocabulary: the same product again, its epilogue
+// writes G = p - q of the piece (and its transpose), then dH += G W and dW = G^T H as two products of the same kernel.
+// Rows are the tokens; in every product the m axis is the one that is contiguous in what the epilogue writes (a lane holds 4 consecutive m).
+#include "gemm_nt.h"
+
+#include <math.h>
+
+namespace cs {
+namespace {
+using namespace nt;
+
+constexpr int KD_MAX_TOP = 1024;
+constexpr int NO_ID = 0x7fffffff;
+enum RowState { ROW_SKIP = 0, ROW_COUNT = 1, ROW_BAD = 2 };
+
+template <int KIND> struct Elem;
+template <> struct Elem<BF16> { typedef __bf16 T; static constexpr float G_SCALE = 1.f; };
+// fp16 holds 2^-24 at least: G, whose entries are p (down to 1 / vocab) and p - q, in [-1, 1], is kept times 2^14
+template <> struct Elem<FP16> { typedef _Float16 T; static constexpr float G_SCALE = 16384.f; };
+template <> struct Elem<FP32> { typedef float T; static constexpr float G_SCALE = 1.f; };
+
+// what the forward pass leaves for the backward pass
+struct Saved {
+    float2* norm;      // [rows] maximum of z, 1 / sum exp((z - maximum) / T)
+    int* state;        // [rows] RowState
+    float* inv_count;  // [1]
+    int* ids;          // [rows][top] ascending, each id once, NO_ID behind the last
+    float* q;          // [rows][top] (distillation)
+    float* z;          // [rows][top]
+};
+
+// the listed ids of a row that fall into [from, from + size): positions lo .. hi of its ascending list
+__device__ __forceinline__ int2 listed_range(const int* ids, int top, int from, int size) {
+    int lo = 0, hi = top;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (ids[mid] < from) lo = mid + 1;
+        else hi = mid;
+    }
+    int end = lo;
+    hi = top;
+    while (end < hi) {
+        const int mid = (end + hi) >> 1;
+        if (ids[mid] - from < size) end = mid + 1;
+        else hi = mid;
+    }
+    return make_int2(lo, end);
+}
+
+// ---- forward: maximum and sum of exponentials of a tile's rows, and the listed z ---------------------------------------------------
+struct NormEpi {
+    float2* part;      // [rows][tiles_m]
+    float* z;          // [rows][top]
+    const int* ids;
+    int rows, vocab, top;
+    float c;           // log2(e) / T
+    template <class R>
+    __device__ __forceinline__ void operator()(const Problem& p, Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF]) const {
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / R::WAVES_N, wn = wave % R::WAVES_N;
+        const int m0 = t.m * R::TILE_M, n0 = t.n * R::TILE_N;
+        float2* join = (float2*)lds;                                     // [WAVES_M][TILE_N]
+        int2* range = (int2*)(lds + R::WAVES_M * R::TILE_N * 8);         // [TILE_N]
+        for (int i = tid; i < R::TILE_N; i += R::THREADS)
+            range[i] = n0 + i < rows ? listed_range(ids + (int64_t)(n0 + i) * top, top, m0, R::TILE_M) : make_int2(0, 0);
+        const int g4 = (lane >> 4) * 4;
+#pragma unroll
+        for (int j = 0; j < R::NF; ++j) {
+            float m = -INFINITY, s = 0.f;
+#pragma unroll
+            for (int i = 0; i < R::MF; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (m0 + R::row0(wm, i) + g4 + r >= vocab) acc[i][j][r] = -INFINITY;
+                    m = fmaxf(m, acc[i][j][r]);
+                }
+            m = fmaxf(m, __shfl_xor(m, 16));
+            m = fmaxf(m, __shfl_xor(m, 32));
+            const float at = m == -INFINITY ? 0.f : m;                   // no value above -inf: the sum is 0, not NaN
+#pragma unroll
+            for (int i = 0; i < R::MF; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[i][j][r] - at) * c);
+            s += __shfl_xor(s, 16);
+            s += __shfl_xor(s, 32);
+            if (lane < 16) join[wm * R::TILE_N + R::col0(wn, j) + lane] = make_float2(m, s);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < R::NF; ++j) {
+            const int col = R::col0(wn, j) + (lane & 15), n = n0 + col;
+            const int2 at = range[col];
+            for (int e = at.x; e < at.y; ++e) {
+                const int want = ids[(int64_t)n * top + e] - m0 - g4;
+                float v = 0.f;
+                bool mine = false;
+#pragma unroll
+                for (int i = 0; i < R::MF; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (want == R::row0(wm, i) + r) {
+                            v = acc[i][j][r];
+                            mine = true;
+                        }
+                if (mine) z[(int64_t)n * top + e] = v;
+            }
+        }
+        for (int i = tid; i < R::TILE_N; i += R::THREADS) {
+            if (n0 + i >= rows) continue;
+            float m = -INFINITY, s = 0.f;
+#pragma unroll
+            for (int w = 0; w < R::WAVES_M; ++w) m = fmaxf(m, join[w * R::TILE_N + i].x);
+            const float at = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int w = 0; w < R::WAVES_M; ++w) {
+                const float2 v = join[w * R::TILE_N + i];
+                s += v.x == -INFINITY ? v.y : v.y * __builtin_amdgcn_exp2f((v.x - at) * c);
+            }
+            part[(int64_t)(n0 + i) * p.tiles_m + t.m] = make_float2(m, s);
+        }
+    }
+};
+
+// ---- backward: G = p - q of a piece of the vocabulary, and its transpose ----------------------------------------------------------
+template <int KIND>
+struct GradEpi {
+    typedef typename Elem<KIND>::T T;
+    T* g;              // [padded rows][pitch_g]
+    T* gt;             // [piece][pitch_gt] or NULL
+    int64_t pitch_g, pitch_gt;
+    Saved s;
+    int rows, from, size, top;     // this piece: ids from .. from + size
+    float c;
+    bool listed_q;                 // distillation: q is in s.q; else 1
+    template <class R>
+    __device__ __forceinline__ void operator()(const Problem& p, Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF]) const {
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / R::WAVES_N, wn = wave % R::WAVES_N;
+        const int m0 = t.m * R::TILE_M, n0 = t.n * R::TILE_N, g4 = (lane >> 4) * 4;
+#pragma unroll
+        for (int j = 0; j < R::NF; ++j) {
+            const int n = n0 + R::col0(wn, j) + (lane & 15);
+            const int state = n < rows ? s.state[n] : ROW_SKIP;
+            const float2 norm = n < rows ? s.norm[n] : make_float2(0.f, 0.f);
+            const float inv = state == ROW_BAD ? __builtin_nanf("") : norm.y * Elem<KIND>::G_SCALE;
+#pragma unroll
+            for (int i = 0; i < R::MF; ++i) {
+                const int m = m0 + R::row0(wm, i) + g4;
+                T v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float e = __builtin_amdgcn_exp2f((acc[i][j][r] - norm.x) * c) * inv;
+                    v[r] = (T)(state == ROW_SKIP || m + r >= size ? 0.f : e);
+                }
+                struct alignas(4 * sizeof(T)) Four { T v[4]; };
+                *(Four*)(g + (int64_t)n * pitch_g + m) = Four{{v[0], v[1], v[2], v[3]}};
+                if (gt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) gt[(int64_t)(m + r) * pitch_gt + n] = v[r];
+            }
+        }
+        wait_loads<0>();                                                 // this wave's stores are done ...
+        barrier();                                                       // ... and everybody's: the listed entries go over them
+        for (int i = tid; i < R::TILE_N; i += R::THREADS) {
+            const int n = n0 + i;
+            if (n >= rows || s.state[n] != ROW_COUNT) continue;
+            const float2 norm = s.norm[n];
+            const int64_t row = (int64_t)n * top;
+            const int2 at = listed_range(s.ids + row, top, from + m0, R::TILE_M);
+            for (int e = at.x; e < at.y; ++e) {
+                const int m = s.ids[row + e] - from;
+                const float q = listed_q ? s.q[row + e] : 1.f;
+                const float v = __builtin_amdgcn_exp2f((s.z[row + e] - norm.x) * c) * norm.y - q;
+                const T out = (T)(v * Elem<KIND>::G_SCALE);
+                g[(int64_t)n * pitch_g + m] = out;
+                if (gt) gt[(int64_t)m * pitch_gt + n] = out;
+            }
+        }
+    }
+};
+
+// ---- dH: fp32 sums over the pieces ------------------------------------------------------------------------------------------------
+struct SumEpi {
+    float* out;        // [splits][rows][width]
+    int rows, width;
+    bool add;
+    template <class R>
+    __device__ __forceinline__ void operator()(const Problem& p, Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF]) const {
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / R::WAVES_N, wn = wave % R::WAVES_N;
+        const int m0 = t.m * R::TILE_M, n0 = t.n * R::TILE_N, g4 = (lane >> 4) * 4;
+        const bool wide = (width & 3) == 0;
+#pragma unroll
+        for (int j = 0; j < R::NF; ++j) {
+            const int n = n0 + R::col0(wn, j) + (lane & 15);
+            if (n >= rows) continue;
+            float* to = out + ((int64_t)t.split * rows + n) * width;
+#pragma unroll
+            for (int i = 0; i < R::MF; ++i) {
+                const int m = m0 + R::row0(wm, i) + g4;
+                if (wide) {
+                    if (m < width) *(f32x4*)(to + m) = add ? *(const f32x4*)(to + m) + acc[i][j] : acc[i][j];
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (m + r < width) to[m + r] = add ? to[m + r] + acc[i][j][r] : acc[i][j][r];
+                }
+            }
+        }
+    }
+};
+
+// ---- dW: one rounding ---------------------------------------------------------------------------------------------------------------
+template <int KIND>
+struct OutEpi {
+    typedef typename Elem<KIND>::T T;
+    T* out;            // [rows of n][width]
+    int rows, width;
+    const float* scale;
+    template <class R>
+    __device__ __forceinline__ void operator()(const Problem& p, Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF]) const {
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / R::WAVES_N, wn = wave % R::WAVES_N;
+        const int m0 = t.m * R::TILE_M, n0 = t.n * R::TILE_N, g4 = (lane >> 4) * 4;
+        const bool wide = (width & 3) == 0;
+        const float f = *scale;
+        struct alignas(4 * sizeof(T)) Four { T v[4]; };
+#pragma unroll
+        for (int j = 0; j < R::NF; ++j) {
+            const int n = n0 + R::col0(wn, j) + (lane & 15);
+            if (n >= rows) continue;
+            T* to = out + (int64_t)n * width;
+#pragma unroll
+            for (int i = 0; i < R::MF; ++i) {
+                const int m = m0 + R::row0(wm, i) + g4;
+                T v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = (T)(acc[i][j][r] * f);
+                if (wide) {
+                    if (m < width) *(Four*)(to + m) = Four{{v[0], v[1], v[2], v[3]}};
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (m + r < width) to[m + r] = v[r];
+                }
+            }
+        }
+    }
+};
+
+template <class R, class EPI>
+__global__ __launch_bounds__(R::THREADS) void product_kernel(Problem p, EPI epi) {
+    __shared__ __attribute__((aligned(1024))) char lds[R::LDS_BYTES];
+    const Tile t = tile_of(blockIdx.x, p);
+    f32x4 acc[R::MF][R::NF];
+    R::run(p, t, lds, acc);
+    epi.template operator()<R>(p, t, lds, acc);
+}
+
+template <int KIND> using Large = Ring<KIND, 256, 256, 2, 4, 2>;
+template <int KIND> using Middle = Ring<KIND, 128, 128, 2, 2, 2>;
+template <int KIND> using Flat = Ring<KIND, 128, 32, 4, 1, 4>;
+
+enum Shape { LARGE, MIDDLE, FLAT };
+struct ShapeSize { int m, n; };
+constexpr ShapeSize SHAPES[3] = {{256, 256}, {128, 128}, {128, 32}};
+
+Shape shape_for(int64_t m, int64_t n) {
+    const int64_t large = ((m + 255) / 256) * ((n + 255) / 256);
+    if (n <= 64) return FLAT;
+    return large >= 192 ? LARGE : MIDDLE;
+}
+
+struct Cut { int splits, per; };
+// k in so many runs that the tiles fill the 256 CUs about twice, of 4 slabs at least
+Cut cut_for(int64_t m, int64_t n, int kbytes, Shape sh, int most) {
+    const int64_t tiles = ((m + SHAPES[sh].m - 1) / SHAPES[sh].m) * ((n + SHAPES[sh].n - 1) / SHAPES[sh].n);
+    const int slabs = (kbytes + 127) / 128;
+    int64_t splits = tiles >= 256 ? 1 : (512 + tiles - 1) / tiles;
+    if (splits > slabs / 4) splits = slabs / 4;
+    if (splits > most) splits = most;
+    if (splits < 1) splits = 1;
+    const int per = (int)((slabs + splits - 1) / splits);
+    return {(slabs + per - 1) / per, per};
+}
+
+template <int KIND, class EPI>
+int launch_product(hipStream_t st, Shape sh, const Operand& a, const Operand& b, int kbytes, Cut cut, const EPI& epi) {
+    Problem p{a, b, kbytes, nullptr, nullptr, 0, 0, (int)((a.rows + SHAPES[sh].m - 1) / SHAPES[sh].m), (int)((b.rows + SHAPES[sh].n - 1) / SHAPES[sh].n), cut.splits, cut.per};
+    const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+    CS_REQUIRE(blocks > 0 && blocks < (int64_t)1 << 31, "head loss: too many tiles");
+    const dim3 grid((unsigned)blocks);
+    if (sh == LARGE) product_kernel<Large<KIND>, EPI><<<grid, Large<KIND>::THREADS, 0, st>>>(p, epi);
+    else if (sh == MIDDLE) product_kernel<Middle<KIND>, EPI><<<grid, Middle<KIND>::THREADS, 0, st>>>(p, epi);
+    else product_kernel<Flat<KIND>, EPI><<<grid, Flat<KIND>::THREADS, 0, st>>>(p, epi);
+    CS_HIP(hipGetLastError());
+    return CS_OK;
+}
+
+// ---- rows ---------------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ int64_t id_at(const void* ids, int bits, int64_t i) {
+    return bits == 64 ? ((const int64_t*)ids)[i] : (int64_t)((const int*)ids)[i];
+}
+
+__global__ __launch_bounds__(256) void target_rows_kernel(const void* ids, int bits, int64_t pitch, int64_t rows, int64_t vocab, int64_t ignore, Saved s) {
+    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (n >= rows) return;
+    const int64_t t = id_at(ids, bits, n * pitch);
+    const bool skip = t == ignore, good = !skip && t >= 0 && t < vocab;
+    s.state[n] = skip ? ROW_SKIP : good ? ROW_COUNT : ROW_BAD;
+    s.ids[n] = good ? (int)t : NO_ID;
+    s.z[n] = 0.f;
+}
+
+__device__ __forceinline__ float teacher_at(const void* p, int type, int64_t i) {
+    if (type == CS_TYPE_BF16) return (float)((const __bf16*)p)[i];
+    if (type == CS_TYPE_FP16) return (float)((const _Float16*)p)[i];
+    return ((const float*)p)[i];
+}
+
+// One block per row: q = softmax(teacher / T) and sum q log q in 64 bits, the ids sorted, the mass of an id that comes twice joined.
+__global__ __launch_bounds__(256) void teacher_rows_kernel(const void* ids, int bits, int64_t ids_pitch, const void* teacher, int type, int64_t teacher_pitch,
+                                                           int top, int64_t vocab, double inv_t, double* entropy, Saved s) {
+    __shared__ unsigned long long key[KD_MAX_TOP];       // id, place in the row
+    __shared__ float mass[KD_MAX_TOP];                   // by place in the row
+    __shared__ int head[2][KD_MAX_TOP];                  // how many different ids up to here
+    __shared__ double sums[4][2];
+    __shared__ float most[4];
+    __shared__ int bad;
+    const int64_t n = blockIdx.x;
+    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 63, wave = tid >> 6, waves = threads >> 6;
+    int size = 1;
+    while (size < top) size *= 2;
+    if (tid == 0) bad = 0;
+    __syncthreads();
+    float m = -INFINITY;
+    for (int i = tid; i < size; i += threads) {
+        const int64_t id = i < top ? id_at(ids, bits, n * ids_pitch + i) : -1;
+        const float l = i < top ? teacher_at(teacher, type, n * teacher_pitch + i) : 0.f;
+        const bool live = id >= 0 && l != -INFINITY;
+        if (live && id >= vocab) bad = 1;
+        key[i] = live ? ((unsigned long long)(id < vocab ? id : vocab) << 32) | (unsigned)i : ~0ull;
+        if (i < top) mass[i] = live ? l : -INFINITY;
+        if (live) m = fmaxf(m, l);
+    }
+#pragma unroll
+    for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+    if (lane == 0) most[wave] = m;
+    __syncthreads();
+    m = most[0];
+    for (int w = 1; w < waves; ++w) m = fmaxf(m, most[w]);
+    double total = 0.0, cross = 0.0;                     // sum e, sum e log e;  e = exp((l - m) / T)
+    for (int i = tid; i < top; i += threads) {
+        const float l = mass[i];
+        if (l == -INFINITY) continue;
+        const double x = ((double)l - (double)m) * inv_t, e = exp(x);
+        total += e;
+        cross += e > 0.0 ? e * x : e;                    // e log e -> 0 with e
+    }
+#pragma unroll
+    for (int x = 32; x; x >>= 1) {
+        total += __shfl_xor(total, x);
+        cross += __shfl_xor(cross, x);
+    }
+    if (lane == 0) {
+        sums[wave][0] = total;
+        sums[wave][1] = cross;
+    }
+    __syncthreads();
+    total = cross = 0.0;
+    for (int w = 0; w < waves; ++w) {
+        total += sums[w][0];
+        cross += sums[w][1];
+    }
+    const bool some = total != 0.0;                      // NaN counts
+    if (tid == 0) {
+        s.state[n] = bad ? ROW_BAD : some ? ROW_COUNT : ROW_SKIP;
+        entropy[n] = some ? cross / total - log(total) : 0.0;
+    }
+    for (int i = tid; i < top; i += threads) {
+        const float l = mass[i];
+        mass[i] = l == -INFINITY ? 0.f : (float)(exp(((double)l - (double)m) * inv_t) / total);
+    }
+    for (int width = 2; width <= size; width *= 2)       // bitonic
+        for (int step = width >> 1; step; step >>= 1) {
+            __syncthreads();
+            for (int i = tid; i < size; i += threads) {
+                const int o = i ^ step;
+                if (o > i) {
+                    const unsigned long long a = key[i], b = key[o];
+                    if ((a > b) == ((i & width) == 0)) {
+                        key[i] = b;
+                        key[o] = a;
+                    }
+                }
+            }
+        }
+    __syncthreads();
+    for (int i = tid; i < size; i += threads) head[0][i] = key[i] != ~0ull && (i == 0 || (key[i - 1] >> 32) != (key[i] >> 32)) ? 1 : 0;
+    int from = 0;
+    for (int step = 1; step < size; step *= 2, from ^= 1) {
+        __syncthreads();
+        for (int i = tid; i < size; i += threads) head[from ^ 1][i] = head[from][i] + (i >= step ? head[from][i - step] : 0);
+    }
+    __syncthreads();
+    const int used = head[from][size - 1];
+    for (int i = tid; i < size; i += threads) {
+        const bool first = key[i] != ~0ull && (i == 0 || (key[i - 1] >> 32) != (key[i] >> 32));
+        if (!first) continue;
+        float q = 0.f;
+        const unsigned id = (unsigned)(key[i] >> 32);
+        for (int k = i; k < size && (unsigned)(key[k] >> 32) == id; ++k) q += mass[(unsigned)key[k]];
+        const int64_t to = n * top + head[from][i] - 1;
+        s.ids[to] = (int64_t)id < vocab ? (int)id : NO_ID;
+        s.q[to] = q;
+        s.z[to] = 0.f;
+    }
+    for (int i = tid; i < top; i += threads)
+        if (i >= used) {
+            s.ids[n * top + i] = NO_ID;
+            s.q[n * top + i] = 0.f;
+            s.z[n * top + i] = 0.f;
+        }
+}
+
+// A wave per row: joins the tiles' maxima and sums, in 64 bits, into the row's loss.
+__global__ __launch_bounds__(256) void row_loss_kernel(const float2* part, int tiles, int64_t rows, int top, bool listed_q, float c, double t, const double* entropy,
+                                                       Saved s, double* losses, float* out) {
+    const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (n >= rows) return;
+    const float2* row = part + n * tiles;
+    float m = -INFINITY;
+    for (int i = lane; i < tiles; i += 64) m = fmaxf(m, row[i].x);
+#pragma unroll
+    for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+    const float at = m == -INFINITY ? 0.f : m;
+    double sum = 0.0, named = 0.0;
+    for (int i = lane; i < tiles; i += 64) {
+        const float2 v = row[i];
+        sum += v.x == -INFINITY ? (double)v.y : (double)v.y * (double)__builtin_amdgcn_exp2f((v.x - at) * c);
+    }
+    for (int i = lane; i < top; i += 64)
+        if (s.ids[n * top + i] != NO_ID) {
+            const float q = listed_q ? s.q[n * top + i] : 1.f;
+            if (q > 0.f || q != q) named += (double)q * (double)s.z[n * top + i];
+        }
+#pragma unroll
+    for (int x = 32; x; x >>= 1) {
+        sum += __shfl_xor(sum, x);
+        named += __shfl_xor(named, x);
+    }
+    if (lane == 0) {
+        const int state = s.state[n];
+        const double h = listed_q ? entropy[n] : 0.0;
+        double loss = t * t * (h + log(sum) + ((double)m - named) / t);
+        if (state == ROW_SKIP) loss = 0.0;
+        if (state == ROW_BAD) loss = (double)__builtin_nanf("");
+        s.norm[n] = make_float2(m, (float)(1.0 / sum));
+        losses[n] = loss;
+        if (out) out[n] = (float)loss;
+    }
+}
+
+// one block: the sum over the rows in a fixed order
+__global__ __launch_bounds__(1024) void reduce_loss_kernel(const double* losses, const int* state, int64_t rows, bool mean, float* loss, float* inv_count) {
+    __shared__ double sums[16];
+    __shared__ int counts[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    double sum = 0.0;
+    int count = 0;
+    for (int64_t n = tid; n < rows; n += 1024) {
+        sum += losses[n];
+        count += state[n] != ROW_SKIP;
+    }
+#pragma unroll
+    for (int x = 32; x; x >>= 1) {
+        sum += __shfl_xor(sum, x);
+        count += __shfl_xor(count, x);
+    }
+    if (lane == 0) {
+        sums[wave] = sum;
+        counts[wave] = count;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        sum = 0.0;
+        count = 0;
+        for (int w = 0; w < 16; ++w) {
+            sum += sums[w];
+            count += counts[w];
+        }
+        const double inv = mean ? 1.0 / (double)(count > 0 ? count : 1) : 1.0;
+        if (loss) *loss = (float)(sum * inv);
+        *inv_count = (float)inv;
+    }
+}
+
+// One block: the factor of every row.  dH of row n is to_h[n] (G W)_n; dW sums in_w[n] h_n, |in_w| <= 1, and is multiplied by *w_scale: a
+// gradient per row is divided by the largest, so that fp16 copies of h keep their range.  Rows that do not count get 0 by selection.
+__global__ __launch_bounds__(1024) void row_scale_kernel(const float* grad, int64_t stride, bool per_row, const int* state, const float* inv_count, int64_t rows,
+                                                         float t, float inv_g, float* to_h, float* in_w, float* w_scale) {
+    __shared__ float most[16];
+    const int tid = threadIdx.x;
+    float big = 0.f;
+    if (per_row) {
+        for (int64_t n = tid; n < rows; n += 1024)
+            if (state[n] != ROW_SKIP) big = fmaxf(big, fabsf(grad[n * stride]));
+#pragma unroll
+        for (int x = 32; x; x >>= 1) big = fmaxf(big, __shfl_xor(big, x));
+        if ((tid & 63) == 0) most[tid >> 6] = big;
+        __syncthreads();
+        big = most[0];
+        for (int w = 1; w < 16; ++w) big = fmaxf(big, most[w]);
+    }
+    const float one = per_row ? 1.f : *grad * *inv_count, f = t * inv_g;
+    for (int64_t n = tid; n < rows; n += 1024) {
+        const bool live = state[n] != ROW_SKIP;
+        const float g = per_row ? grad[n * stride] : one;
+        to_h[n] = live ? g * f : 0.f;
+        in_w[n] = !live ? 0.f : !per_row ? 1.f : big == 0.f ? g : g / big;
+    }
+    if (tid == 0) *w_scale = (per_row ? (big == 0.f ? 1.f : big) : one) * f;
+}
+
+// src [rows][cols] (element pitch) -> dst [cols][pitch], columns of dst behind the rows zero up to `padded`; row n times scale[n] (NULL: 1; 0 selects 0)
+template <class T>
+__global__ __launch_bounds__(256) void transpose_kernel(const T* src, int64_t src_pitch, int64_t rows, int64_t cols, T* dst, int64_t dst_pitch, int64_t padded,
+                                                        const float* scale) {
+    __shared__ T tile[64][64 + 4 / sizeof(T) + 1];
+    const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
+    const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+    for (int i = y; i < 64; i += 4) {
+        T v = (T)0.f;
+        if (r0 + i < rows && c0 + x < cols) {
+            v = src[(r0 + i) * src_pitch + c0 + x];
+            if (scale) {
+                const float f = scale[r0 + i];
+                v = f == 0.f ? (T)0.f : f == 1.f ? v : (T)((float)v * f);
+            }
+        }
+        tile[i][x] = v;
+    }
+    __syncthreads();
+    for (int i = y; i < 64; i += 4)
+        if (c0 + i < cols && r0 + x < padded) dst[(c0 + i) * dst_pitch + r0 + x] = tile[x][i];
+}
+
+// src [rows][cols] -> dst [rows][pitch], zeros behind the columns
+template <class T>
+__global__ __launch_bounds__(256) void copy_rows_kernel(const T* src, int64_t src_pitch, int64_t cols, T* dst, int64_t pitch) {
+    for (int64_t c = threadIdx.x; c < pitch; c += 256) dst[(int64_t)blockIdx.x * pitch + c] = c < cols ? src[(int64_t)blockIdx.x * src_pitch + c] : (T)0.f;
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void hidden_grad_kernel(const float* sums, int splits, int64_t rows, int64_t width, const float* scale, T* out) {
+    const int64_t n = blockIdx.x;
+    const float f = scale[n];
+    for (int64_t c = threadIdx.x; c < width; c += 256) {
+        float v = 0.f;
+        for (int s = 0; s < splits; ++s) v += sums[((int64_t)s * rows + n) * width + c];
+        out[n * width + c] = (T)(f == 0.f ? 0.f : v * f);
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void zero_kernel(T* out, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) out[i] = (T)0.f;
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------------------------
+struct Arena {
+    char* base;
+    size_t at = 0;
+    template <class T> T* take(size_t count) {
+        T* p = base ? (T*)(base + at) : nullptr;
+        at += (count * sizeof(T) + 255) & ~(size_t)255;
+        return p;
+    }
+};
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+int type_bytes(int type) { return type == CS_TYPE_FP32 ? 4 : 2; }
+
+Saved carve_saved(const cs_head_loss& h, void* base, size_t* bytes) {
+    Arena a{(char*)base};
+    Saved s;
+    const size_t n = (size_t)h.rows, k = (size_t)h.top;
+    s.norm = a.take<float2>(n);
+    s.state = a.take<int>(n);
+    s.inv_count = a.take<float>(1);
+    s.ids = a.take<int>(n * k);
+    s.z = a.take<float>(n * k);
+    s.q = a.take<float>(h.kind == CS_HEAD_DISTILLATION ? n * k : 0);
+    *bytes = a.at;
+    return s;
+}
+
+// whether the product can read an operand where it lies
+bool in_place(const void* p, int64_t pitch, int64_t width, int size) {
+    return ((uintptr_t)p & 15) == 0 && (pitch * size) % 16 == 0 && (width * size) % 16 == 0 && pitch * size < ((int64_t)1 << 28);
+}
+
+struct Plan {
+    size_t bytes;
+    char *hidden, *weight;                 // padded copies, NULL where the tensor is read in place
+    int64_t hidden_pitch, weight_pitch;    // bytes
+    float2* part;
+    double *losses, *entropy;
+    int64_t padded, piece;                 // rows and vocabulary of a piece, rounded up to 256
+    Cut cut;                               // of the sums of dH over the first piece; a shorter last piece adds to fewer of them
+    Shape dh_shape;
+    char *g, *gt, *wt, *ht;
+    float *sums, *to_h, *in_w, *w_scale;
+};
+
+constexpr int64_t PIECE_BYTES = (int64_t)512 << 20;      // of G
+
+Plan make_plan(const cs_head_loss& h, int backward, void* base) {
+    Plan p{};
+    Arena a{(char*)base};
+    const int size = type_bytes(h.type);
+    const int64_t width_pitch = up(h.width * size, 128);
+    const bool hin = in_place(h.hidden, h.hidden_pitch, h.width, size), win = in_place(h.weight, h.weight_pitch, h.width, size);
+    p.hidden_pitch = hin ? h.hidden_pitch * size : width_pitch;
+    p.weight_pitch = win ? h.weight_pitch * size : width_pitch;
+    if (!hin) p.hidden = a.take<char>((size_t)(h.rows * width_pitch));
+    if (!win) p.weight = a.take<char>((size_t)(h.vocab * width_pitch));
+    if (!backward) {
+        const Shape sh = shape_for(h.vocab, h.rows);
+        p.part = a.take<float2>((size_t)(h.rows * ((h.vocab + SHAPES[sh].m - 1) / SHAPES[sh].m)));
+        p.losses = a.take<double>((size_t)h.rows);
+        p.entropy = a.take<double>((size_t)(h.kind == CS_HEAD_DISTILLATION ? h.rows : 0));
+    } else if (h.rows) {
+        p.padded = up(h.rows, 256);
+        p.piece = PIECE_BYTES / (p.padded * size) / 256 * 256;
+        if (p.piece < 256) p.piece = 256;
+        if (p.piece > up(h.vocab, 256)) p.piece = up(h.vocab, 256);
+        p.g = a.take<char>((size_t)(p.padded * p.piece * size));
+        p.to_h = a.take<float>((size_t)h.rows);
+        p.in_w = a.take<float>((size_t)h.rows);
+        p.w_scale = a.take<float>(1);
+        if (backward & 1) {
+            p.dh_shape = shape_for(h.width, h.rows);
+            p.cut = cut_for(h.width, h.rows, (int)((p.piece < h.vocab ? p.piece : up(h.vocab, 64)) * size), p.dh_shape, 64);
+            p.wt = a.take<char>((size_t)(h.width * p.piece * size));
+            p.sums = a.take<float>((size_t)p.cut.splits * h.rows * h.width);
+        }
+        if (backward & 2) {
+            p.gt = a.take<char>((size_t)(p.padded * p.piece * size));
+            p.ht = a.take<char>((size_t)(h.width * p.padded * size));
+        }
+    }
+    p.bytes = a.at;
+    return p;
+}
+
+template <class T>
+void copy_rows(hipStream_t st, const void* src, int64_t pitch, int64_t rows, int64_t cols, void* dst, int64_t dst_pitch_bytes) {
+    copy_rows_kernel<T><<<dim3((unsigned)rows), 256, 0, st>>>((const T*)src, pitch, cols, (T*)dst, dst_pitch_bytes / (int64_t)sizeof(T));
+}
+template <class T>
+void transpose(hipStream_t st, const void* src, int64_t pitch, int64_t rows, int64_t cols, void* dst, int64_t dst_pitch, int64_t padded, const float* scale) {
+    transpose_kernel<T><<<dim3((unsigned)((padded + 63) / 64), (unsigned)((cols + 63) / 64)), 256, 0, st>>>((const T*)src, pitch, rows, cols, (T*)dst, dst_pitch, padded, scale);
+}
+
+int check_head(const cs_head_loss* h) {
+    CS_REQUIRE(h, "head loss: NULL descriptor");
+    CS_REQUIRE(h->rows >= 0 && h->rows < (int64_t)1 << 26 && h->vocab >= 1 && h->vocab < (int64_t)1 << 30 && h->width >= 1 && h->width < (int64_t)1 << 21,
+               "head loss: rows %lld, vocab %lld, width %lld out of range", (long long)h->rows, (long long)h->vocab, (long long)h->width);
+    CS_REQUIRE(h->type >= CS_TYPE_BF16 && h->type <= CS_TYPE_FP32, "head loss: unknown type %d", h->type);
+    CS_REQUIRE(h->kind == CS_HEAD_CROSS_ENTROPY || h->kind == CS_HEAD_DISTILLATION, "head loss: unknown kind %d", h->kind);
+    CS_REQUIRE(h->reduction >= CS_REDUCE_NONE && h->reduction <= CS_REDUCE_SUM, "head loss: unknown reduction %d", h->reduction);
+    CS_REQUIRE(h->ids_bits == 32 || h->ids_bits == 64, "head loss: ids of %d bits", h->ids_bits);
+    if (h->kind == CS_HEAD_DISTILLATION) {
+        CS_REQUIRE(h->top >= 1 && h->top <= KD_MAX_TOP, "head loss: %d teacher logits per row: 1..%d are supported", h->top, KD_MAX_TOP);
+        CS_REQUIRE(h->teacher_type >= CS_TYPE_BF16 && h->teacher_type <= CS_TYPE_FP32, "head loss: unknown teacher type %d", h->teacher_type);
+        CS_REQUIRE(h->temperature > 0.0 && h->temperature < 1e30, "head loss: temperature %g", h->temperature);
+    } else {
+        CS_REQUIRE(h->top == 1 && h->temperature == 1.0, "head loss: the cross entropy has top = 1 and temperature = 1");
+    }
+    CS_REQUIRE(h->hidden_pitch >= h->width || h->rows <= 1, "head loss: hidden rows overlap (pitch %lld < width %lld)", (long long)h->hidden_pitch, (long long)h->width);
+    CS_REQUIRE(h->weight_pitch >= h->width || h->vocab <= 1, "head loss: weight rows overlap (pitch %lld < width %lld)", (long long)h->weight_pitch, (long long)h->width);
+    return CS_OK;
+}
+
+template <int KIND>
+int forward(const cs_head_loss& h, const Plan& p, const Saved& s, float* row_losses, float* loss, hipStream_t st) {
+    typedef typename Elem<KIND>::T T;
+    const int size = sizeof(T);
+    const bool kd = h.kind == CS_HEAD_DISTILLATION;
+    if (h.rows) {
+        if (kd) {
+            const int threads = h.top <= 64 ? 64 : h.top <= 128 ? 128 : 256;
+            teacher_rows_kernel<<<dim3((unsigned)h.rows), threads, 0, st>>>(h.ids, h.ids_bits, h.ids_pitch, h.teacher, h.teacher_type, h.teacher_pitch, h.top, h.vocab,
+                                                                           1.0 / h.temperature, p.entropy, s);
+        } else {
+            target_rows_kernel<<<dim3((unsigned)((h.rows + 255) / 256)), 256, 0, st>>>(h.ids, h.ids_bits, h.ids_pitch, h.rows, h.vocab, h.ignore_index, s);
+        }
+        if (p.hidden) copy_rows<T>(st, h.hidden, h.hidden_pitch, h.rows, h.width, p.hidden, p.hidden_pitch);
+        if (p.weight) copy_rows<T>(st, h.weight, h.weight_pitch, h.vocab, h.width, p.weight, p.weight_pitch);
+        const Operand a{p.weight ? p.weight : (const char*)h.weight, p.weight_pitch, h.vocab}, b{p.hidden ? p.hidden : (const char*)h.hidden, p.hidden_pitch, h.rows};
+        const int kbytes = (int)(p.hidden || p.weight ? up(h.width * size, 16) : h.width * size);
+        const float c = (float)(1.4426950408889634 / h.temperature);
+        const Shape sh = shape_for(h.vocab, h.rows);
+        const int tiles = (int)((h.vocab + SHAPES[sh].m - 1) / SHAPES[sh].m);
+        const NormEpi epi{p.part, s.z, s.ids, (int)h.rows, (int)h.vocab, h.top, c};
+        if (int rc = launch_product<KIND>(st, sh, a, b, kbytes, Cut{1, (kbytes + 127) / 128}, epi)) return rc;
+        row_loss_kernel<<<dim3((unsigned)((h.rows + 3) / 4)), 256, 0, st>>>(p.part, tiles, h.rows, h.top, kd, c, h.temperature, p.entropy, s, p.losses, row_losses);
+    }
+    reduce_loss_kernel<<<1, 1024, 0, st>>>(p.losses, s.state, h.rows, h.reduction == CS_REDUCE_MEAN, loss, s.inv_count);
+    CS_HIP(hipGetLastError());
+    return CS_OK;
+}
+
+template <int KIND>
+int backward(const cs_head_loss& h, const Plan& p, const Saved& s, const float* grad, int64_t grad_stride, void* gh, void* gw, hipStream_t st) {
+    typedef typename Elem<KIND>::T T;
+    const int size = sizeof(T);
+    if (!h.rows) {
+        if (gw) zero_kernel<T><<<1024, 256, 0, st>>>((T*)gw, h.vocab * h.width);
+        CS_HIP(hipGetLastError());
+        return CS_OK;
+    }
+    const bool kd = h.kind == CS_HEAD_DISTILLATION;
+    const float c = (float)(1.4426950408889634 / h.temperature);
+    row_scale_kernel<<<1, 1024, 0, st>>>(grad, grad_stride, h.reduction == CS_REDUCE_NONE, s.state, s.inv_count, h.rows, (float)h.temperature, 1.f / Elem<KIND>::G_SCALE,
+                                         p.to_h, p.in_w, p.w_scale);
+    if (p.hidden) copy_rows<T>(st, h.hidden, h.hidden_pitch, h.rows, h.width, p.hidden, p.hidden_pitch);
+    if (p.weight) copy_rows<T>(st, h.weight, h.weight_pitch, h.vocab, h.width, p.weight, p.weight_pitch);
+    const int kbytes = (int)(p.hidden || p.weight ? up(h.width * size, 16) : h.width * size);
+    if (gw) transpose<T>(st, h.hidden, h.hidden_pitch, h.rows, h.width, p.ht, p.padded, up(h.rows, 32), p.in_w);
+    for (int64_t from = 0; from < h.vocab; from += p.piece) {
+        const int64_t len = h.vocab - from < p.piece ? h.vocab - from : p.piece, klen = up(len, 64);
+        const Operand a{(p.weight ? p.weight : (const char*)h.weight) + from * p.weight_pitch, p.weight_pitch, len};
+        const Operand b{p.hidden ? p.hidden : (const char*)h.hidden, p.hidden_pitch, h.rows};
+        const GradEpi<KIND> grad_epi{(T*)p.g, gw ? (T*)p.gt : nullptr, p.piece, p.padded, s, (int)h.rows, (int)from, (int)len, h.top, c, kd};
+        if (int rc = launch_product<KIND>(st, shape_for(len, h.rows), a, b, kbytes, Cut{1, (kbytes + 127) / 128}, grad_epi)) return rc;
+        if (gh) {
+            transpose<T>(st, (const T*)h.weight + from * h.weight_pitch, h.weight_pitch, len, h.width, p.wt, p.piece, klen, nullptr);
+            const int kb = (int)(klen * size), slabs = (kb + 127) / 128;
+            const Cut cut{(slabs + p.cut.per - 1) / p.cut.per, p.cut.per};
+            const SumEpi epi{p.sums, (int)h.rows, (int)h.width, from != 0};
+            if (int rc = launch_product<KIND>(st, p.dh_shape, Operand{p.wt, p.piece * size, h.width}, Operand{p.g, p.piece * size, h.rows}, kb, cut, epi)) return rc;
+        }
+        if (gw) {
+            const int kb = (int)(up(h.rows, 32) * size);
+            const OutEpi<KIND> epi{(T*)gw + from * h.width, (int)len, (int)h.width, p.w_scale};
+            if (int rc = launch_product<KIND>(st, shape_for(h.width, len), Operand{p.ht, p.padded * size, h.width}, Operand{p.gt, p.padded * size, len}, kb,
+                                              Cut{1, (kb + 127) / 128}, epi))
+                return rc;
+        }
+    }
+    if (gh) hidden_grad_kernel<T><<<dim3((unsigned)h.rows), 256, 0, st>>>(p.sums, p.cut.splits, h.rows, h.width, p.to_h, (T*)gh);
+    CS_HIP(hipGetLastError());
+    return CS_OK;
+}
+
+}  // namespace
+}  // namespace cs
+
+extern "C" {
+using namespace cs;
+
+size_t cs_head_loss_saved_bytes(const cs_head_loss* h) {
+    if (check_head(h) != CS_OK) return 0;
+    size_t bytes;
+    carve_saved(*h, nullptr, &bytes);
+    return bytes;
+}
+
+size_t cs_head_loss_workspace_bytes(const cs_head_loss* h, int backward) {
+    if (check_head(h) != CS_OK) return 0;
+    return make_plan(*h, backward, nullptr).bytes;
+}
+
+int cs_head_loss_forward(const cs_head_loss* h, float* row_losses, float* loss, void* saved, size_t saved_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int rc = check_head(h)) return rc;
+    CS_REQUIRE((h->hidden || !h->rows) && h->weight && (h->ids || !h->rows) && (h->teacher || !h->rows || h->kind == CS_HEAD_CROSS_ENTROPY) && saved && workspace,
+               "head loss: NULL pointer");
+    size_t need;
+    const Saved s = carve_saved(*h, saved, &need);
+    const Plan p = make_plan(*h, 0, workspace);
+    if (saved_bytes < need || workspace_bytes < p.bytes) {
+        set_error("head loss: workspace of %zu / %zu bytes, %zu / %zu are needed", saved_bytes, workspace_bytes, need, p.bytes);
+        return CS_ERR_WORKSPACE;
+    }
+    const double nvd = 2.0 * (double)h->rows * (double)h->vocab * (double)h->width;
+    ProfScope prof(K_HEAD_LOSS, (hipStream_t)stream, nvd, (double)(h->rows + h->vocab) * h->width * type_bytes(h->type));
+    if (h->type == CS_TYPE_BF16) return forward<nt::BF16>(*h, p, s, row_losses, loss, (hipStream_t)stream);
+    if (h->type == CS_TYPE_FP16) return forward<nt::FP16>(*h, p, s, row_losses, loss, (hipStream_t)stream);
+    return forward<nt::FP32>(*h, p, s, row_losses, loss, (hipStream_t)stream);
+}
+
+int cs_head_loss_backward(const cs_head_loss* h, const void* saved, size_t saved_bytes, const float* grad, int64_t grad_stride, void* grad_hidden, void* grad_weight,
+                          void* workspace, size_t workspace_bytes, void* stream) {
+    if (int rc = check_head(h)) return rc;
+    const int want = (grad_hidden ? 1 : 0) | (grad_weight ? 2 : 0);
+    if (!want) return CS_OK;
+    CS_REQUIRE(((uintptr_t)grad_hidden & 15) == 0 && ((uintptr_t)grad_weight & 15) == 0, "head loss: gradients are written at 16-byte aligned addresses");
+    CS_REQUIRE((h->hidden || !h->rows) && h->weight && saved && (grad || !h->rows) && workspace, "head loss: NULL pointer");
+    size_t need;
+    const Saved s = carve_saved(*h, const_cast<void*>(saved), &need);
+    const Plan p = make_plan(*h, want, workspace);
+    if (saved_bytes < need || workspace_bytes < p.bytes) {
+        set_error("head loss: workspace of %zu / %zu bytes, %zu / %zu are needed", saved_bytes, workspace_bytes, need, p.bytes);
+        return CS_ERR_WORKSPACE;
+    }
+    const double nvd = 2.0 * (double)h->rows * (double)h->vocab * (double)h->width;
+    ProfScope prof(K_HEAD_LOSS, (hipStream_t)stream, nvd * ((want & 1) + (want >> 1)), 2.0 * (double)(h->rows + h->vocab) * h->width * type_bytes(h->type));
+    if (h->type == CS_TYPE_BF16) return backward<nt::BF16>(*h, p, s, grad, grad_stride, grad_hidden, grad_weight, (hipStream_t)stream);
+    if (h->type == CS_TYPE_FP16) return backward<nt::FP16>(*h, p, s, grad, grad_stride, grad_hidden, grad_weight, (hipStream_t)stream);
+    return backward<nt::FP32>(*h, p, s, grad, grad_stride, grad_hidden, grad_weight, (hipStream_t)stream);
+}
+
+}  // extern "C"

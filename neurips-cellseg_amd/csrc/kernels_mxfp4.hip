@@ -1,0 +1,310 @@
+// gfx950 (MI355X): the microscaled 4-bit format (OCP MX, MXFP4) - quantisation, dequantisation and the linear layer on it.
+// 32 consecutive values along the inner axis share one scale 2^(s - 127), s = floor(log2 max|x|) - 2 + 127 clamped at 0 (one e8m0 byte);
+// each value is x / scale rounded to e2m1 (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives), ties to the even code, above 6 to 6.  A block
+// with an infinity or NaN has the scale byte 0xff, which stands for NaN.  Two codes a byte, the even one in the low half; a row that ends
+// inside a block is filled up with zeros.
+#include "gemm_nt.h"
+
+namespace cs {
+namespace {
+using namespace nt;
+
+template <int TYPE> struct Value;
+template <> struct Value<CS_TYPE_BF16> { typedef __bf16 T; };
+template <> struct Value<CS_TYPE_FP16> { typedef _Float16 T; };
+template <> struct Value<CS_TYPE_FP32> { typedef float T; };
+
+// 8 values from column c of a row of `width`
+template <class T>
+__device__ __forceinline__ void load8(const T* row, int64_t c, int64_t width, bool wide, float (&v)[8]) {
+    if (wide && c + 8 <= width) {
+        struct alignas(16) Eight { T v[8]; };
+        const Eight e = *(const Eight*)(row + c);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)e.v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < width ? (float)row[c + i] : 0.f;
+    }
+}
+
+// 8 values of a lane, 4 lanes a block -> their codes; `scale`: the block's byte, the same in the 4 lanes
+__device__ __forceinline__ unsigned encode8(const float (&v)[8], unsigned* scale) {
+    unsigned most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, __builtin_bit_cast(unsigned, v[i]) & 0x7fffffffu);
+    most = max(most, (unsigned)__shfl_xor((int)most, 1));
+    most = max(most, (unsigned)__shfl_xor((int)most, 2));
+    const int field = (int)(most >> 23);                                 // the exponent's field of the largest
+    if (field == 255) {
+        *scale = 255u;
+        return 0u;
+    }
+    const int s = field > 2 ? field - 2 : 0;
+    *scale = (unsigned)s;
+    const float by = __builtin_bit_cast(float, (unsigned)(254 - s) << 23);   // 2^(127 - s): s <= 252, a normal number
+    unsigned out = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float a = fabsf(v[i] * by);
+        const unsigned code = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.f);
+        out |= (code | (__builtin_bit_cast(unsigned, v[i]) >> 31 << 3)) << (4 * i);
+    }
+    return out;
+}
+
+// place of the scale byte of (row, block) in the order that the product reads (gemm_nt.h: a word per pair of slabs, row and chunk column)
+__device__ __forceinline__ int64_t tile_place(int64_t row, int64_t block, int64_t rows) {
+    return (((block >> 4) * rows + row) * 4 + (block & 3)) * 4 + ((block >> 2) & 3);
+}
+
+// 4 lanes a block.  TILED: scales in the product's order over `rows_tiled` rows, blocks up to a multiple of 16 and rows behind the last with
+// scale 1 and no codes; else [rows][blocks]
+template <class T, bool TILED>
+__global__ __launch_bounds__(256) void quantise_kernel(const T* x, int64_t pitch, int64_t rows, int64_t width, int64_t blocks, bool wide, uint8_t* codes, uint8_t* scales,
+                                                       int64_t rows_tiled) {
+    const int64_t per = TILED ? (blocks + 15) / 16 * 16 : blocks, total = (TILED ? rows_tiled : rows) * per * 4;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t b = i >> 2, row = b / per, block = b - row * per;
+        const int part = (int)(i & 3);
+        const bool in = !TILED || (row < rows && block < blocks);
+        float v[8];
+        if (in) load8(x + row * pitch, block * 32 + part * 8, width, wide, v);
+        else
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = 0.f;
+        unsigned scale;
+        const unsigned code = encode8(v, &scale);
+        if (in) *(unsigned*)(codes + (row * blocks + block) * 16 + part * 4) = code;
+        if (part == 0) scales[TILED ? tile_place(row, block, rows_tiled) : row * blocks + block] = (uint8_t)(in ? scale : 127u);
+    }
+}
+
+// [rows][blocks] scales -> the product's order
+__global__ __launch_bounds__(256) void tile_scales_kernel(const uint8_t* scales, int64_t rows, int64_t blocks, uint8_t* out, int64_t rows_tiled) {
+    const int64_t total = rows_tiled * ((blocks + 15) / 16) * 4;         // words of 4 blocks: 4 h' + g, h' = 0..3
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t g = i & 3, row = (i >> 2) % rows_tiled, pair = (i >> 2) / rows_tiled;
+        unsigned word = 0;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            const int64_t block = pair * 16 + h * 4 + g;
+            word |= (row < rows && block < blocks ? (unsigned)scales[row * blocks + block] : 127u) << (8 * h);
+        }
+        ((unsigned*)out)[i] = word;
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void dequantise_kernel(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t width, int64_t blocks, bool wide, T* out) {
+    const int64_t total = rows * blocks * 4;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t b = i >> 2, row = b / blocks, c = (b - row * blocks) * 32 + (i & 3) * 8;
+        const unsigned code = *(const unsigned*)(codes + i * 4), s = scales[b];
+        const float by = s == 255u ? __builtin_nanf("") : ldexpf(1.f, (int)s - 127);
+        struct alignas(16) Eight { T v[8]; } e;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const unsigned q = code >> (4 * k), m = q & 7u;
+            // e2m1: exponent m / 2, mantissa m & 1; 0 and 1 (0.5) have no implicit one
+            const float a = m < 2u ? 0.5f * (float)m : __builtin_bit_cast(float, (((m >> 1) + 126u) << 23) | ((m & 1u) << 22));
+            e.v[k] = (T)((q & 8u ? -a : a) * by);
+        }
+        T* to = out + row * width + c;
+        if (wide && c + 8 <= width) *(Eight*)to = e;
+        else
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (c + k < width) to[k] = e.v[k];
+    }
+}
+
+// ---- the linear layer: y[n][m] = sum_k x[n][k] w[m][k], m the outputs ------------------------------------------------------------------
+template <class T>
+struct LinearEpi {
+    T* out;            // [rows][outputs]
+    int rows, outputs;
+    template <class R>
+    __device__ __forceinline__ void operator()(const Problem& p, Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF]) const {
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / R::WAVES_N, wn = wave % R::WAVES_N;
+        const int m0 = t.m * R::TILE_M, n0 = t.n * R::TILE_N, g4 = (lane >> 4) * 4;
+        const bool wide = (outputs & 3) == 0;
+        struct alignas(4 * sizeof(T)) Four { T v[4]; };
+#pragma unroll
+        for (int j = 0; j < R::NF; ++j) {
+            const int n = n0 + R::col0(wn, j) + (lane & 15);
+            if (n >= rows) continue;
+            T* to = out + (int64_t)n * outputs;
+#pragma unroll
+            for (int i = 0; i < R::MF; ++i) {
+                const int m = m0 + R::row0(wm, i) + g4;
+                T v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = (T)acc[i][j][r];
+                if (wide) {
+                    if (m < outputs) *(Four*)(to + m) = Four{{v[0], v[1], v[2], v[3]}};
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (m + r < outputs) to[m + r] = v[r];
+                }
+            }
+        }
+    }
+};
+
+template <class R, class EPI>
+__global__ __launch_bounds__(R::THREADS) void linear_kernel(Problem p, EPI epi) {
+    __shared__ __attribute__((aligned(1024))) char lds[R::LDS_BYTES];
+    const Tile t = tile_of(blockIdx.x, p);
+    f32x4 acc[R::MF][R::NF];
+    R::run(p, t, lds, acc);
+    epi.template operator()<R>(p, t, lds, acc);
+}
+
+typedef Ring<E2M1, 256, 256, 2, 4, 2> Large;
+typedef Ring<E2M1, 128, 128, 2, 2, 2> Middle;
+typedef Ring<E2M1, 128, 32, 4, 1, 4> Flat;
+
+template <class R, class T>
+int launch_linear(hipStream_t st, Problem p, LinearEpi<T> epi) {
+    p.tiles_m = (int)((p.a.rows + R::TILE_M - 1) / R::TILE_M);
+    p.tiles_n = (int)((p.b.rows + R::TILE_N - 1) / R::TILE_N);
+    p.splits = 1;
+    p.slabs_per_split = (p.kbytes + 127) / 128;
+    const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n;
+    CS_REQUIRE(blocks < (int64_t)1 << 31, "mxfp4 linear: too many tiles");
+    linear_kernel<R, LinearEpi<T>><<<dim3((unsigned)blocks), R::THREADS, 0, st>>>(p, epi);
+    CS_HIP(hipGetLastError());
+    return CS_OK;
+}
+
+unsigned grid_for(int64_t items) {
+    const int64_t blocks = (items + 255) / 256;
+    return (unsigned)(blocks < 8192 ? blocks : 8192);
+}
+
+struct LinearPlan {
+    size_t bytes;
+    uint8_t *codes, *scales_x, *scales_w;
+    int64_t blocks, rows_x, rows_w;
+};
+LinearPlan make_plan(int64_t rows, int64_t width, int64_t outputs, void* base) {
+    LinearPlan p{};
+    p.blocks = (width + 31) / 32;
+    p.rows_x = (rows + 255) / 256 * 256;
+    p.rows_w = (outputs + 255) / 256 * 256;
+    const int64_t tiled = (p.blocks + 15) / 16 * 16;
+    size_t at = 0;
+    auto take = [&](int64_t n) {
+        uint8_t* q = base ? (uint8_t*)base + at : nullptr;
+        at += ((size_t)n + 255) & ~(size_t)255;
+        return q;
+    };
+    p.codes = take(rows * p.blocks * 16);
+    p.scales_x = take(p.rows_x * tiled);
+    p.scales_w = take(p.rows_w * tiled);
+    p.bytes = at;
+    return p;
+}
+
+int check_sizes(int64_t rows, int64_t width, int type, const char* what) {
+    CS_REQUIRE(rows >= 0 && rows < (int64_t)1 << 30 && width >= 1 && width < (int64_t)1 << 24, "%s: rows %lld, width %lld out of range", what, (long long)rows,
+               (long long)width);
+    CS_REQUIRE(type >= CS_TYPE_BF16 && type <= CS_TYPE_FP32, "%s: unknown type %d", what, type);
+    return CS_OK;
+}
+
+template <class T>
+bool reads_wide(const void* x, int64_t pitch) {
+    return ((uintptr_t)x & 15) == 0 && (pitch * (int64_t)sizeof(T)) % 16 == 0;
+}
+
+template <class T>
+int quantise(const void* x, int64_t pitch, int64_t rows, int64_t width, uint8_t* codes, uint8_t* scales, hipStream_t st) {
+    const int64_t blocks = (width + 31) / 32;
+    quantise_kernel<T, false><<<grid_for(rows * blocks * 4), 256, 0, st>>>((const T*)x, pitch, rows, width, blocks, reads_wide<T>(x, pitch), codes, scales, 0);
+    CS_HIP(hipGetLastError());
+    return CS_OK;
+}
+template <class T>
+int dequantise(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t width, void* out, hipStream_t st) {
+    const int64_t blocks = (width + 31) / 32;
+    dequantise_kernel<T><<<grid_for(rows * blocks * 4), 256, 0, st>>>(codes, scales, rows, width, blocks, reads_wide<T>(out, width), (T*)out);
+    CS_HIP(hipGetLastError());
+    return CS_OK;
+}
+template <class T>
+int linear(const void* x, int64_t pitch, int64_t rows, int64_t width, const uint8_t* codes, const uint8_t* scales, int64_t outputs, void* y, const LinearPlan& p,
+           hipStream_t st) {
+    quantise_kernel<T, true><<<grid_for(p.rows_x * ((p.blocks + 15) / 16) * 64), 256, 0, st>>>((const T*)x, pitch, rows, width, p.blocks, reads_wide<T>(x, pitch), p.codes,
+                                                                                             p.scales_x, p.rows_x);
+    tile_scales_kernel<<<grid_for(p.rows_w * ((p.blocks + 15) / 16) * 4), 256, 0, st>>>(scales, outputs, p.blocks, p.scales_w, p.rows_w);
+    CS_HIP(hipGetLastError());
+    Problem q{};
+    q.a = Operand{(const char*)codes, p.blocks * 16, outputs};
+    q.b = Operand{(const char*)p.codes, p.blocks * 16, rows};
+    q.kbytes = (int)(p.blocks * 16);
+    q.scales_a = (const unsigned*)p.scales_w;
+    q.scales_b = (const unsigned*)p.scales_x;
+    q.rows_a = p.rows_w;
+    q.rows_b = p.rows_x;
+    const LinearEpi<T> epi{(T*)y, (int)rows, (int)outputs};
+    if (rows <= 64) return launch_linear<Flat>(st, q, epi);
+    if (((outputs + 255) / 256) * ((rows + 255) / 256) >= 192) return launch_linear<Large>(st, q, epi);
+    return launch_linear<Middle>(st, q, epi);
+}
+
+}  // namespace
+}  // namespace cs
+
+extern "C" {
+using namespace cs;
+
+int cs_mxfp4_quantize(const void* x, int64_t pitch, int64_t rows, int64_t width, int type, uint8_t* codes, uint8_t* scales, void* stream) {
+    if (int rc = check_sizes(rows, width, type, "mxfp4 quantize")) return rc;
+    if (!rows) return CS_OK;
+    CS_REQUIRE(x && codes && scales, "mxfp4 quantize: NULL pointer");
+    CS_REQUIRE(((uintptr_t)codes & 3) == 0, "mxfp4 quantize: codes start at a multiple of 4 bytes");
+    ProfScope prof(K_MXFP4, (hipStream_t)stream, 0, (double)rows * width * (type == CS_TYPE_FP32 ? 4.53 : 2.53));
+    if (type == CS_TYPE_BF16) return quantise<__bf16>(x, pitch, rows, width, codes, scales, (hipStream_t)stream);
+    if (type == CS_TYPE_FP16) return quantise<_Float16>(x, pitch, rows, width, codes, scales, (hipStream_t)stream);
+    return quantise<float>(x, pitch, rows, width, codes, scales, (hipStream_t)stream);
+}
+
+int cs_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t width, int type, void* out, void* stream) {
+    if (int rc = check_sizes(rows, width, type, "mxfp4 dequantize")) return rc;
+    if (!rows) return CS_OK;
+    CS_REQUIRE(out && codes && scales, "mxfp4 dequantize: NULL pointer");
+    CS_REQUIRE(((uintptr_t)codes & 3) == 0, "mxfp4 dequantize: codes start at a multiple of 4 bytes");
+    ProfScope prof(K_MXFP4, (hipStream_t)stream, 0, (double)rows * width * (type == CS_TYPE_FP32 ? 4.53 : 2.53));
+    if (type == CS_TYPE_BF16) return dequantise<__bf16>(codes, scales, rows, width, out, (hipStream_t)stream);
+    if (type == CS_TYPE_FP16) return dequantise<_Float16>(codes, scales, rows, width, out, (hipStream_t)stream);
+    return dequantise<float>(codes, scales, rows, width, out, (hipStream_t)stream);
+}
+
+size_t cs_mxfp4_linear_workspace_bytes(int64_t rows, int64_t width, int64_t outputs) {
+    if (check_sizes(rows, width, CS_TYPE_BF16, "mxfp4 linear") || check_sizes(outputs, width, CS_TYPE_BF16, "mxfp4 linear")) return 0;
+    return make_plan(rows, width, outputs, nullptr).bytes;
+}
+
+int cs_mxfp4_linear(const void* x, int64_t pitch, int64_t rows, int64_t width, int type, const uint8_t* codes, const uint8_t* scales, int64_t outputs, void* y,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+    if (int rc = check_sizes(rows, width, type, "mxfp4 linear")) return rc;
+    if (int rc = check_sizes(outputs, width, type, "mxfp4 linear")) return rc;
+    if (!rows || !outputs) return CS_OK;
+    CS_REQUIRE(x && y && codes && scales && workspace, "mxfp4 linear: NULL pointer");
+    CS_REQUIRE(((uintptr_t)codes & 15) == 0 && ((uintptr_t)y & 15) == 0, "mxfp4 linear: codes and output start at a multiple of 16 bytes");
+    const LinearPlan p = make_plan(rows, width, outputs, workspace);
+    if (workspace_bytes < p.bytes) {
+        set_error("mxfp4 linear: workspace of %zu bytes, %zu are needed", workspace_bytes, p.bytes);
+        return CS_ERR_WORKSPACE;
+    }
+    const double size = type == CS_TYPE_FP32 ? 4.0 : 2.0;
+    ProfScope prof(K_MXFP4, (hipStream_t)stream, 2.0 * rows * width * outputs, size * rows * (width + outputs) + 0.53 * outputs * width);
+    if (type == CS_TYPE_BF16) return linear<__bf16>(x, pitch, rows, width, codes, scales, outputs, y, p, (hipStream_t)stream);
+    if (type == CS_TYPE_FP16) return linear<_Float16>(x, pitch, rows, width, codes, scales, outputs, y, p, (hipStream_t)stream);
+    return linear<float>(x, pitch, rows, width, codes, scales, outputs, y, p, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,100 @@
+"""Refusals of the head losses and the 4-bit operators, and the descriptor's layout: nothing here runs on a GPU."""
+import ctypes as C
+import os
+import subprocess
+
+import pytest
+import torch
+
+import cellseg_amd as ca
+from cellseg_amd import _lib
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+H, W, T = torch.randn(4, 8), torch.randn(10, 8), torch.zeros(4, dtype=torch.int64)
+IDS, LOGITS = torch.zeros(4, 3, dtype=torch.int64), torch.zeros(4, 3)
+
+
+def test_head_descriptor_layout_matches_the_c_header(tmp_path):
+    fields = [f[0] for f in _lib.HeadLoss._fields_]
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "cellseg_hip.h"\nint main(void) {\n  printf("%zu", sizeof(cs_head_loss));\n'
+                   + "".join(f'  printf(" %zu", offsetof(cs_head_loss, {f}));\n' for f in fields) + "  return 0;\n}\n")
+    exe = tmp_path / "layout"
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    got = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [C.sizeof(_lib.HeadLoss)] + [getattr(_lib.HeadLoss, f).offset for f in fields]
+
+
+@pytest.mark.parametrize("call,error", [
+    (lambda: ca.linear_cross_entropy(H, W, T), ca.CellSegHipError),                                   # CPU tensors: no fallback
+    (lambda: ca.linear_cross_entropy(H, W.bfloat16(), T), TypeError),
+    (lambda: ca.linear_cross_entropy(H.double(), W.double(), T), TypeError),
+    (lambda: ca.linear_cross_entropy(H, W, T.float()), TypeError),
+    (lambda: ca.linear_cross_entropy(H, W[:, :7], T), ValueError),
+    (lambda: ca.linear_cross_entropy(H, W[:0], T), ValueError),
+    (lambda: ca.linear_cross_entropy(H, W[None], T), ValueError),
+    (lambda: ca.linear_cross_entropy(H, W, T, reduction="batchmean"), ValueError),
+    (lambda: ca.linear_distillation(H, W, IDS, LOGITS), ca.CellSegHipError),
+    (lambda: ca.LinearCrossEntropyLoss(reduction="x"), ValueError),
+    (lambda: ca.LinearDistillationLoss(temperature=0.0), ValueError),
+    (lambda: ca.mxfp4_quantize(H), ca.CellSegHipError),
+    (lambda: ca.mxfp4_quantize(H.double()), TypeError),
+    (lambda: ca.mxfp4_quantize(H[:, :0]), ValueError),
+    (lambda: ca.mxfp4_quantize(H.clone().requires_grad_()), ValueError),
+    (lambda: ca.mxfp4_linear(H, W), TypeError),
+    (lambda: ca.MXFP4Tensor(torch.zeros(3, 15, dtype=torch.uint8), torch.zeros(3, 1, dtype=torch.uint8), 32), ValueError),
+    (lambda: ca.MXFP4Tensor(torch.zeros(3, 16, dtype=torch.uint8), torch.zeros(3, 2, dtype=torch.uint8), 32), ValueError),
+    (lambda: ca.MXFP4Tensor(torch.zeros(3, 16), torch.zeros(3, 1, dtype=torch.uint8), 32), ValueError),
+    (lambda: ca.MXFP4Tensor(torch.zeros(3, 16, dtype=torch.uint8), torch.zeros(3, 1, dtype=torch.uint8), 32, torch.int8), TypeError),
+    (lambda: ca.mxfp4_linear(H[:, :7], ca.MXFP4Tensor(torch.zeros(3, 16, dtype=torch.uint8), torch.zeros(3, 1, dtype=torch.uint8), 8)), ValueError),
+    (lambda: ca.mxfp4_linear(H.clone().requires_grad_(), ca.MXFP4Tensor(torch.zeros(3, 16, dtype=torch.uint8), torch.zeros(3, 1, dtype=torch.uint8), 8)), ValueError),
+    (lambda: ca.mxfp4_linear(H, ca.MXFP4Tensor(torch.zeros(3, 16, dtype=torch.uint8), torch.zeros(3, 1, dtype=torch.uint8), 8)), ca.CellSegHipError),
+])
+def test_refusals(call, error):
+    with pytest.raises(error):
+        call()
+
+
+def head(**over):
+    d = dict(hidden=4096, weight=8192, ids=4096, teacher=None, hidden_pitch=8, weight_pitch=8, ids_pitch=1, teacher_pitch=0, rows=4, vocab=10, width=8, ignore_index=-100,
+             temperature=1.0, type=0, kind=0, reduction=1, ids_bits=64, teacher_type=0, top=1)
+    d.update(over)
+    return _lib.HeadLoss(**d)
+
+
+@pytest.mark.parametrize("over", [dict(rows=-1), dict(rows=1 << 26), dict(vocab=0), dict(vocab=1 << 30), dict(width=0), dict(width=1 << 21), dict(type=3), dict(kind=2), dict(reduction=3),
+                                  dict(ids_bits=16), dict(top=2), dict(temperature=2.0), dict(kind=1, top=0), dict(kind=1, top=1025), dict(kind=1, temperature=0.0),
+                                  dict(kind=1, temperature=float("nan")), dict(kind=1, teacher_type=4), dict(hidden_pitch=7), dict(weight_pitch=7)])
+def test_the_c_entry_refuses(over):
+    """Bad descriptors and NULL pointers are refused before anything is launched (no GPU is needed to see that)."""
+    h = head(**over)
+    assert _lib.lib.cs_head_loss_saved_bytes(C.byref(h)) == 0 and _lib.lib.cs_head_loss_workspace_bytes(C.byref(h), 3) == 0
+    assert _lib.lib.cs_head_loss_forward(C.byref(h), None, 4096, 4096, 1 << 40, 4096, 1 << 40, None) == -1
+    assert _lib.lib.cs_head_loss_backward(C.byref(h), 4096, 1 << 40, 4096, 0, 4096, 4096, 4096, 1 << 40, None) == -1
+
+
+def test_the_c_entry_refuses_small_workspaces_and_null():
+    h = head()
+    saved, ws = _lib.lib.cs_head_loss_saved_bytes(C.byref(h)), _lib.lib.cs_head_loss_workspace_bytes(C.byref(h), 0)
+    assert saved > 0 and ws > 0
+    assert _lib.lib.cs_head_loss_forward(C.byref(h), None, 4096, 4096, saved - 1, 4096, ws, None) == -3
+    assert _lib.lib.cs_head_loss_forward(C.byref(h), None, 4096, 4096, saved, 4096, ws - 1, None) == -3
+    assert _lib.lib.cs_head_loss_forward(C.byref(h), None, 4096, None, saved, 4096, ws, None) == -1
+    back = _lib.lib.cs_head_loss_workspace_bytes(C.byref(h), 3)
+    assert _lib.lib.cs_head_loss_backward(C.byref(h), 4096, saved, 4096, 0, 4096, 4096, 4096, back - 1, None) == -3
+    assert _lib.lib.cs_head_loss_backward(C.byref(h), 4096, saved, None, 0, 4096, 4096, 4096, back, None) == -1
+    assert _lib.lib.cs_head_loss_backward(C.byref(h), 4096, saved, 4096, 0, 4100, 4096, 4096, back, None) == -1
+    assert _lib.lib.cs_mxfp4_quantize(4096, 8, 4, 0, 0, 4096, 4096, None) == -1
+    assert _lib.lib.cs_mxfp4_quantize(4096, 8, 4, 8, 5, 4096, 4096, None) == -1
+    assert _lib.lib.cs_mxfp4_quantize(None, 8, 4, 8, 0, 4096, 4096, None) == -1
+    assert _lib.lib.cs_mxfp4_dequantize(4098, 4096, 4, 8, 0, 4096, None) == -1
+    size = _lib.lib.cs_mxfp4_linear_workspace_bytes(4, 8, 6)
+    assert size > 0 and _lib.lib.cs_mxfp4_linear(4096, 8, 4, 8, 0, 4096, 4096, 6, 4096, 4096, size - 1, None) == -3
+    assert _lib.lib.cs_mxfp4_linear(4096, 8, 4, 8, 0, 4100, 4096, 6, 4096, 4096, size, None) == -1
+
+
+def test_workspaces_of_no_rows():
+    h = head(rows=0, hidden=None)
+    assert _lib.lib.cs_head_loss_saved_bytes(C.byref(h)) > 0
+    for backward in range(4):
+        assert _lib.lib.cs_head_loss_workspace_bytes(C.byref(h), backward) == 0

@@ -13,6 +13,7 @@
 #include "cs_common.h"
 
 #include <type_traits>
+#include <utility>
 
 namespace cs {
 namespace nt {
@@ -27,7 +28,7 @@ enum Kind { BF16 = 0, FP16 = 1, FP32 = 2, E2M1 = 3 };
 
 struct Operand {
     const char* ptr;       // row 0
-    int64_t pitch;         // bytes between rows: a multiple of 16, below 2^23 (256 rows then fit a 32-bit offset)
+    int64_t pitch;         // bytes between rows: a multiple of 16, below 2^25 (128 rows then fit a 32-bit offset)
     int64_t rows;          // >= 1
 };
 
@@ -66,6 +67,16 @@ __device__ __forceinline__ void barrier() {
     asm volatile("" ::: "memory");
 }
 
+// a barrier behind this wave's LDS accesses, with its global loads and stores left under way
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    barrier();
+}
+
+// between a wave's LDS writes and its reads of what other lanes of it wrote, and back: the wave's LDS accesses run in order, but the compiler
+// sees one lane and may exchange those that do not meet in it
+__device__ __forceinline__ void wave_sync() { asm volatile("" ::: "memory"); }
+
 // c += a b over one chunk per lane; e2m1: byte SEL of the lanes' scale words (an immediate of the instruction)
 template <int KIND, int SEL>
 __device__ __forceinline__ f32x4 mma(i32x4 a, i32x4 b, f32x4 c, int scale_a, int scale_b) {
@@ -84,19 +95,42 @@ __device__ __forceinline__ f32x4 mma(i32x4 a, i32x4 b, f32x4 c, int scale_a, int
     }
 }
 
-// block id -> (tile_m, tile_n, split).  Blocks go to the 8 XCDs in turn; each XCD gets a contiguous run of tiles, walked in groups of
-// 8 tile rows, so the tiles that run together on an XCD share their operands' slabs in its L2.
+// The same with the sum in place in accumulation registers (the compiler else moves the 256 of a large tile about between its uses).  One
+// instruction (fp32: of element `element`); no other of the next few may touch the same sum, and a reader of the sum waits for the pipe.
+template <int KIND, int SEL>
+__device__ __forceinline__ void mma_in_place(f32x4& c, i32x4 a, i32x4 b, int element, int scale_a, int scale_b) {
+    if constexpr (KIND == BF16) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    else if constexpr (KIND == FP16) asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    else if constexpr (KIND == FP32) asm volatile("v_mfma_f32_16x16x4_f32 %0, %1, %2, %0" : "+a"(c) : "v"(a[element]), "v"(b[element]));
+    else
+        asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%5,0] op_sel_hi:[%6,%6,0] cbsz:4 blgp:4"
+                     : "+a"(c) : "v"(a), "v"(b), "v"(scale_a), "v"(scale_b), "n"(SEL & 1), "n"(SEL >> 1));
+}
+
+// block id -> (tile_m, tile_n, split).  Blocks go to the 8 XCDs in turn and about 256 run at a time.  Of every 256 consecutive tiles an
+// XCD gets 32 in a row; tiles are walked in groups of 8 tile rows, so an XCD's 32 share 8 + 4 operand panels in its L2 and all 256 share
+// 8 + 32 in the memory-side cache.
 struct Tile { int m, n, split; };
 __device__ __forceinline__ Tile tile_of(int id, const Problem& p) {
-    const int per = p.tiles_m * p.tiles_n, total = per * p.splits;
-    const int q = total >> 3, r = total & 7, xcd = id & 7, at = id >> 3;
-    int t = xcd < r ? xcd * (q + 1) + at : r * (q + 1) + (xcd - r) * q + at;
+    const int per = p.tiles_m * p.tiles_n, whole = per * p.splits & ~255;
+    int t = id < whole ? (id & ~255) + (id & 7) * 32 + ((id & 255) >> 3) : id;
     const int split = t / per;
     t -= split * per;
     const int group = t / (8 * p.tiles_n), first = group * 8, height = min(p.tiles_m - first, 8);
     t -= group * 8 * p.tiles_n;
     return {first + t % height, t / height, split};
 }
+
+// a value that the compiler does not carry through a loop in a dozen forms (it spills them): computed again where it is used
+__device__ __forceinline__ int fresh(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+template <class F, int... N>
+__device__ __forceinline__ void each(std::integer_sequence<int, N...>, F f) { (f(std::integral_constant<int, N>()), ...); }
+template <int N, class F>
+__device__ __forceinline__ void each(F f) { each(std::make_integer_sequence<int, N>(), f); }
 
 // What one block multiplies: BM x BN outputs, WM x WN waves, STAGES slabs of both operands in LDS.
 template <int KIND, int BM, int BN, int WM, int WN, int STAGES>
@@ -207,6 +241,292 @@ struct Ring {
         barrier();                                                       // LDS is the epilogue's
     }
 };
+
+// The large tile: 256 x 256 outputs on 4 waves of 128 x 128, one wave per SIMD.  Against 8 waves of 128 x 64 it reads 128 instead of
+// 192 KB of LDS per slab (a CU reads 128 bytes per clock and needs 2048 clocks of matrix instructions per slab), so LDS stays behind the
+// matrix pipe.  A wave multiplies a half slab (64 products, 16 clocks each) while it reads the fragments of the next:
+//   first half of a slab    reads the second half's fragments; FREE: all waves have them, the slab after the next starts over this one
+//   second half             LANDED: the next slab is there for all waves; reads its first half's fragments
+// What bounds this loop is the way from L2 to LDS and the issue of anything between two products: one fetch in front of every fourth
+// product and a read in front of two of five take 1.39 us a slab (the products alone 0.91); all fetches of a slab in a row 1.49, one wait for
+// everything per slab 1.55 (bf16, 4096 x 8192 x 8192: 1545 TFLOP/s).
+// A block takes its tiles one after the other as one stream of slabs: while the epilogue of a tile runs, the first two slabs of the next
+// are under way or there.  The epilogue has the LDS behind LDS_BYTES; it must not wait for the loads in flight.
+template <int KIND, bool TAIL = false>
+struct Wide {
+    static constexpr int KIND_ = KIND, TILE_M = 256, TILE_N = 256, WAVES_M = 2, WAVES_N = 2, THREADS = 256, MF = 8, NF = 8;
+    static constexpr int STAGE_BYTES = 512 * 128, LDS_BYTES = 2 * STAGE_BYTES + (KIND == E2M1 ? 2 * 8192 : 0), LOADS = 16;
+    static constexpr int FREE = 44, LANDED = 23;                // products of a half in front of which the two barriers stand
+    static constexpr int OUT = (64 - FREE + LANDED) / 4;         // of a slab's fetches: how many are out when LANDED is reached
+    static_assert(FREE >= 3 + 38 && LANDED + 38 <= 64 && (64 - FREE) % 4 == 0 && LANDED % 4 == 3 && OUT < LOADS, "");
+    // of a half's 16 reads: how many stand in front of product n, 2 in 5 from product `from` on
+    static __device__ constexpr int reads(int n, int from) { return n <= from ? 0 : ((n - from) * 2 + 3) / 5 > 16 ? 16 : ((n - from) * 2 + 3) / 5; }
+    static_assert(reads(FREE, 3) == 16 && reads(64, LANDED) == 16, "");
+    static __device__ __forceinline__ int row0(int wm, int i) { return wm * 128 + i * 16; }
+    static __device__ __forceinline__ int col0(int wn, int j) { return wn * 128 + j * 16; }
+
+    template <class EPI>
+    static __device__ __forceinline__ void run(const Problem& p, char* lds, const EPI& epi) {
+        const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int wm = wave >> 1, wn = wave & 1;
+        const int tiles = p.tiles_m * p.tiles_n * p.splits, stride = gridDim.x;
+        const int slabs = (p.kbytes + 127) >> 7, pairs = (slabs + 1) >> 1;
+        const std::integral_constant<int, 0> zero;
+        const std::integral_constant<int, 1> one;
+        auto first_of = [&](const Tile& t) { return t.split * p.slabs_per_split; };
+        auto last_of = [&](const Tile& t) { return KIND == E2M1 ? 2 * pairs - 1 : min(slabs, (t.split + 1) * p.slabs_per_split) - 1; };   // e2m1: whole pairs
+
+        // ---- the stream of slabs: waves 0 and 1 fetch A, 2 and 3 B: 128 rows each, 8 rows a fetch
+        const Operand& o = wave < 2 ? p.a : p.b;
+        const unsigned chunk = (unsigned)((lane & 7) ^ (lane >> 3)) * 16u;
+        const unsigned to = lds_address(lds) + (unsigned)wave * 16384u;
+        int fetch_tile = blockIdx.x, fetch_slab = first_of(tile_of(fetch_tile, p)), fetch_last;
+        const char* base;
+        unsigned off[LOADS];
+        auto point = [&](auto again) {                                   // at fetch_tile
+            const Tile t = tile_of(fetch_tile, p);
+            fetch_last = last_of(t);
+            const int64_t r0 = (wave < 2 ? (int64_t)t.m * 256 : (int64_t)t.n * 256) + (wave & 1) * 128;
+            const int64_t from = r0 < o.rows ? r0 : o.rows - 1;
+            const int left = (int)min((int64_t)128, o.rows - from);      // rows that exist
+            base = o.ptr + from * o.pitch;
+            const int row = fresh(lane >> 3);
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const unsigned v = (unsigned)min(i * 8 + row, left - 1) * (unsigned)o.pitch + chunk;
+                if constexpr (again.value) asm volatile("v_mov_b32 %0, %1" : "+v"(off[i]) : "v"(v));   // in place: the loop would else copy all 16 every time
+                else off[i] = v;
+            }
+        };
+        auto advance = [&]() {                                           // behind the last tile the last slab comes again, unread
+            if (fetch_slab < fetch_last) ++fetch_slab;
+            else if (fetch_tile + stride < tiles) {
+                fetch_tile += stride;
+                fetch_slab = first_of(tile_of(fetch_tile, p));
+                point(one);
+            }
+        };
+        // TAIL: k does not end with a slab; where this lane's chunk of the last one lies behind the end it fetches the page of zeros.  A build of
+        // its own, since the branch around each fetch costs 10 %.
+        const char* at;
+        auto aim = [&]() { at = base + (int64_t)fetch_slab * 128; };
+        auto load = [&](int slot, int i) {
+            const unsigned dst = to + (unsigned)(slot * STAGE_BYTES + i * 1024);
+            if (TAIL && fetch_slab * 128 + 128 > p.kbytes) dma16(dst, fetch_slab * 128 + (int)chunk < p.kbytes ? at + off[i] : (const char*)zero_page);
+            else dma16(dst, at + off[i]);
+        };
+
+        // ---- e2m1: the scale words of a pair of slabs, 16 bytes a row, fetched one pair ahead into LDS behind the slabs; 16 words a lane go to
+        // registers before the pair begins
+        int scale[16], scale_tile = blockIdx.x, scale_pair = 0, scale_slot = 0;
+        auto load_scales = [&]() {
+            const Tile t = tile_of(scale_tile, p);
+            const int64_t row = (wave < 2 ? scale_pair * p.rows_a + (int64_t)t.m * 256 : scale_pair * p.rows_b + (int64_t)t.n * 256) + (wave & 1) * 128;
+            const char* from = (const char*)(wave < 2 ? p.scales_a : p.scales_b) + row * 16 + lane * 16;
+            const unsigned dst = lds_address(lds) + (unsigned)(2 * STAGE_BYTES + scale_slot * 8192 + wave * 2048);
+            dma16(dst, from);
+            dma16(dst + 1024, from + 1024);
+            if (++scale_pair == pairs && scale_tile + stride < tiles) {
+                scale_pair = 0;
+                scale_tile += stride;
+            }
+            scale_pair = min(scale_pair, pairs - 1);
+            scale_slot ^= 1;
+        };
+        auto read_scales = [&]() {                                       // of the pair that was fetched last
+            const char* from = lds + 2 * STAGE_BYTES + (scale_slot ^ 1) * 8192 + (lane & 15) * 16 + (lane >> 4) * 4;
+#pragma unroll
+            for (int n = 0; n < 16; ++n) scale[n] = *(const int*)(from + (n < NF ? 4096 + wn * 2048 + n * 256 : wm * 2048 + (n - NF) * 256));
+        };
+
+        int place[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) place[h] = (lane & 15) * 128 + (((h * 4 + (lane >> 4)) ^ (lane & 7)) * 16);
+        const char* sa = lds + wm * 16384;
+        const char* sb = lds + 32768 + wn * 16384;
+        i32x4 a[2][MF], b[2][NF];
+        auto read = [&](int slot, auto h, int n) {                      // the n-th of a half slab's 16 fragments
+            if (n < NF) b[h.value][n] = *(const i32x4*)(sb + slot * STAGE_BYTES + place[h.value] + n * 2048);
+            else a[h.value][n - NF] = *(const i32x4*)(sa + slot * STAGE_BYTES + place[h.value] + (n - NF) * 2048);
+        };
+        f32x4 acc[MF][NF];
+        // 64 products of a half, with before(n) in front of the n-th; the order is kept as it is written
+        auto multiply = [&](auto odd, auto h, auto before) {
+            constexpr int PER = KIND == FP32 ? 4 : 1;                    // fp32: an instruction per element, all 64 products between two of them
+            each<64>([&](auto n) {
+                before(n);
+                __builtin_amdgcn_sched_barrier(0);
+                each<PER>([&](auto q) {
+                    constexpr int N = n.value * PER + q.value, E = N >> 6, I = (N & 63) >> 3, J = N & 7;
+                    mma_in_place<KIND, 2 * odd.value + h.value>(acc[I][J], a[h.value][I], b[h.value][J], E, scale[NF + I], scale[J]);
+                });
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        };
+        int slot = 0;
+        auto step = [&](auto odd) {
+            constexpr bool SCALES = KIND == E2M1 && odd.value == 0;      // 2 more loads in flight when LANDED is reached
+            multiply(odd, zero, [&](auto n) {
+                constexpr int N = n.value, I = (N - FREE) / 4;
+                if constexpr (reads(N + 1, 3) > reads(N, 3)) read(slot, one, reads(N, 3));
+                if constexpr (SCALES && N == 1) load_scales();
+                if constexpr (N == 2) advance();
+                if constexpr (N == FREE - 1) aim();
+                if constexpr (N == FREE) lds_barrier();
+                if constexpr (N > FREE && (N - FREE) % 4 == 3) load(slot, I);
+            });
+            multiply(odd, one, [&](auto n) {
+                constexpr int N = n.value, I = (N + 64 - FREE) / 4;
+                if constexpr ((N + 64 - FREE) % 4 == 3 && I < LOADS) load(slot, I);
+                if constexpr (N == LANDED) {
+                    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OUT + (SCALES ? 2 : 0)) : "memory");
+                    barrier();
+                }
+                if constexpr (reads(N + 1, LANDED) > reads(N, LANDED)) read(slot ^ 1, zero, reads(N, LANDED));
+            });
+            if constexpr (KIND == E2M1 && odd.value == 1) read_scales();
+            slot ^= 1;
+        };
+
+        if constexpr (KIND == E2M1) load_scales();
+        point(zero);
+        aim();
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) load(0, i);
+        advance();
+        aim();
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) load(1, i);
+        wait_loads<LOADS>();
+        barrier();
+        for (int id = blockIdx.x; id < tiles; id += stride) {
+            point(zero);                                                 // again, and the first fragments too: no register but the sums lives through an epilogue
+#pragma unroll
+            for (int n = 0; n < 16; ++n) read(slot, zero, n);
+            if constexpr (KIND == E2M1) read_scales();
+            const Tile t = tile_of(id, p);
+#pragma unroll
+            for (int i = 0; i < MF; ++i)
+#pragma unroll
+                for (int j = 0; j < NF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            int left = last_of(t) - first_of(t) + 1;
+            do {
+                step(zero);
+                if constexpr (KIND == E2M1) step(one);
+                left -= KIND == E2M1 ? 2 : 1;
+                if (left == 0) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");    // the last sums leave the pipe before anything reads them
+            } while (left);
+            epi.template operator()<Wide>(p, t, lds + LDS_BYTES, acc);
+        }
+        wait_loads<0>();
+    }
+};
+
+// the sums of columns `from` on stay in accumulation registers up to here: over branches the compiler else takes all of them out at once and
+// spills (a third of the time of an epilogue)
+template <class R>
+__device__ __forceinline__ void hold(f32x4 (&acc)[R::MF][R::NF], int from) {
+    if constexpr (R::MF * R::NF > 32)
+#pragma unroll
+        for (int i = 0; i < R::MF; ++i)
+#pragma unroll
+            for (int j = 0; j < R::NF; ++j)
+                if (j >= from) asm volatile("" : "+a"(acc[i][j]));
+}
+
+// a sum out of its accumulation registers, here and not earlier: 256 of them read ahead of their use would not fit beside what is live
+__device__ __forceinline__ f32x4 take(const f32x4& sum) {
+    f32x4 v;
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" : "=v"(v) : "0"(sum));
+    return v;
+}
+
+__device__ __forceinline__ void give(f32x4& sum, f32x4 v) { asm volatile("" : "=a"(sum) : "0"(v)); }
+
+// A wave's tile to out[n][m] (m contiguous, `ld` elements between rows), n < rows, m < width: 16-bit rows 16 at a time, 32-bit rows 8 at a time
+// through LDS, so that a store covers whole lines (from registers it would cover runs of 32 or 64 bytes), and past the caches: written the plain
+// way the 33 MB that 256 tiles leave at once push the operands out of L2 (50176 x 4096 x 2048: 1180 TFLOP/s, with whole lines 1260, past the
+// caches 1440).  `value`: sum -> what is stored; `add`: onto what is there.  Rows that are no multiple of 16 bytes go element by element.
+template <class T, int N> struct Stage {         // rows of N elements; chunk c of 16 bytes of row r lies at c ^ r: rows written together meet on no bank
+    static constexpr int ROWS = 32 / (int)sizeof(T), LANES = N * (int)sizeof(T) / 16, BYTES = ROWS * N * (int)sizeof(T);
+    static __device__ __forceinline__ int at(int row, int byte) { return (row * LANES + ((byte >> 4) ^ (row & (LANES - 1)))) * 16 + (byte & 15); }
+};
+template <class R, class T>
+constexpr int stage_bytes() { return R::WAVES_M * R::WAVES_N * Stage<T, R::TILE_M / R::WAVES_M>::BYTES; }
+
+template <class R, class T, class VALUE>
+__device__ __forceinline__ void store_tile(Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF], T* out, int64_t ld, int rows, int width, bool add, VALUE value) {
+    typedef Stage<T, R::TILE_M / R::WAVES_M> S;
+    struct alignas(4 * sizeof(T)) Four { T v[4]; };
+    struct alignas(16) Chunk { T v[16 / sizeof(T)]; };
+    const int tid = fresh(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / R::WAVES_N, wn = wave % R::WAVES_N;
+    const int m = t.m * R::TILE_M + R::row0(wm, 0) + (lane % S::LANES) * (16 / (int)sizeof(T)), g4 = (lane >> 4) * 4, col = lane & 15;
+    const bool wide = (ld * (int64_t)sizeof(T)) % 16 == 0;
+    char* stage = lds + wave * S::BYTES;
+#pragma unroll
+    for (int j = 0; j < R::NF; ++j)
+#pragma unroll
+        for (int part = 0; part < 16; part += S::ROWS) {
+            hold<R>(acc, j);
+#pragma unroll
+            for (int i = 0; i < R::MF; ++i) {
+                const f32x4 v = take(acc[i][j]);
+                const Four f = {{(T)value(v[0]), (T)value(v[1]), (T)value(v[2]), (T)value(v[3])}};
+                if (S::ROWS == 16 || (col & ~(S::ROWS - 1)) == part) *(Four*)(stage + S::at(col & (S::ROWS - 1), (i * 16 + g4) * (int)sizeof(T))) = f;
+            }
+            wave_sync();
+#pragma unroll
+            for (int r = 0; r < S::ROWS; r += 64 / S::LANES) {
+                const int row = r + lane / S::LANES, n = t.n * R::TILE_N + R::col0(wn, j) + part + row;
+                if (row >= S::ROWS || n >= rows || m >= width) continue;
+                Chunk c = *(const Chunk*)(stage + S::at(row, (lane % S::LANES) * 16));
+                T* to = out + (int64_t)n * ld + m;
+                if (wide) {
+                    if (add) {
+                        const Chunk old = *(const Chunk*)to;
+#pragma unroll
+                        for (int e = 0; e < 16 / (int)sizeof(T); ++e) c.v[e] = (T)((float)c.v[e] + (float)old.v[e]);
+                    }
+                    __builtin_nontemporal_store(__builtin_bit_cast(i32x4, c), (i32x4*)to);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16 / (int)sizeof(T); ++e)
+                        if (m + e < width) to[e] = add ? (T)((float)c.v[e] + (float)to[e]) : c.v[e];
+                }
+            }
+            wave_sync();
+        }
+}
+
+// A kernel's body: the LDS that it needs, and its tile (Ring) or tiles (Wide)
+template <class R> struct Persistent { static constexpr bool value = false; };
+template <int KIND, bool TAIL> struct Persistent<Wide<KIND, TAIL>> { static constexpr bool value = true; };
+template <class R, class EPI>
+constexpr int lds_bytes() {
+    return Persistent<R>::value ? R::LDS_BYTES + EPI::template lds<R>() : R::LDS_BYTES > EPI::template lds<R>() ? R::LDS_BYTES : EPI::template lds<R>();
+}
+template <class R, class EPI>
+__device__ __forceinline__ void product(const Problem& p, char* lds, const EPI& epi) {
+    if constexpr (Persistent<R>::value) {
+        R::run(p, lds, epi);
+    } else {
+        const Tile t = tile_of(blockIdx.x, p);
+        f32x4 acc[R::MF][R::NF];
+        R::run(p, t, lds, acc);
+        epi.template operator()<R>(p, t, lds, acc);
+    }
+}
+
+constexpr int CUS = 256;                     // of an MI355X: one block of large tiles each
+
+// Blocks of a launch.  Long tiles go to a block each: they are dealt out as CUs come free, and 1 % of a tile is saved by chaining them (16 tiles of
+// 64 slabs: 1.60 against 1.64 ms chained; 2 tiles of 510 slabs: 1.63 against 1.49 ms, the slowest CU's two).
+template <class R>
+unsigned grid_of(const Problem& p) {
+    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+    return (unsigned)(Persistent<R>::value && p.slabs_per_split < 128 && tiles > CUS ? CUS : tiles);
+}
 
 }  // namespace nt
 }  // namespace cs

@@ -32,101 +32,107 @@ struct Saved {
     int* ids;          // [rows][top] ascending, each id once, NO_ID behind the last
     float* q;          // [rows][top] (distillation)
     float* z;          // [rows][top]
+    uint16_t* starts;  // [rows][starts_pitch] distillation: how many ids of the row lie below 128 t
+    int64_t starts_pitch;
 };
 
-// the listed ids of a row that fall into [from, from + size): positions lo .. hi of its ascending list
-__device__ __forceinline__ int2 listed_range(const int* ids, int top, int from, int size) {
-    int lo = 0, hi = top;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (ids[mid] < from) lo = mid + 1;
-        else hi = mid;
+// Where a row's ascending list of ids has those of a tile's m0 .. m0 + size: positions lo .. hi.  The cross entropy has one id a row; a
+// list has its positions at the multiples of 128 beside it, so that no tile searches.
+template <bool LIST>
+__device__ __forceinline__ int2 listed_range(const Saved& s, int64_t n, int from, int size) {
+    if constexpr (LIST) {
+        const uint16_t* at = s.starts + n * s.starts_pitch + (from >> 7);
+        return make_int2(at[0], at[size >> 7]);
+    } else {
+        return make_int2(0, (unsigned)(s.ids[n] - from) < (unsigned)size ? 1 : 0);
     }
-    int end = lo;
-    hi = top;
-    while (end < hi) {
-        const int mid = (end + hi) >> 1;
-        if (ids[mid] - from < size) end = mid + 1;
-        else hi = mid;
-    }
-    return make_int2(lo, end);
 }
 
 // ---- forward: maximum and sum of exponentials of a tile's rows, and the listed z ---------------------------------------------------
+template <bool LIST>
 struct NormEpi {
     float2* part;      // [rows][tiles_m]
-    float* z;          // [rows][top]
-    const int* ids;
+    Saved s;
     int rows, vocab, top;
     float c;           // log2(e) / T
+    template <class R> static constexpr int lds() { return R::WAVES_M * R::TILE_N * 8; }
     template <class R>
     __device__ __forceinline__ void operator()(const Problem& p, Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF]) const {
-        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / R::WAVES_N, wn = wave % R::WAVES_N;
+        const int tid = fresh(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / R::WAVES_N, wn = wave % R::WAVES_N;
         const int m0 = t.m * R::TILE_M, n0 = t.n * R::TILE_N;
         float2* join = (float2*)lds;                                     // [WAVES_M][TILE_N]
-        int2* range = (int2*)(lds + R::WAVES_M * R::TILE_N * 8);         // [TILE_N]
-        for (int i = tid; i < R::TILE_N; i += R::THREADS)
-            range[i] = n0 + i < rows ? listed_range(ids + (int64_t)(n0 + i) * top, top, m0, R::TILE_M) : make_int2(0, 0);
         const int g4 = (lane >> 4) * 4;
+        hold<R>(acc, 0);
+        int2 range[R::NF];
 #pragma unroll
         for (int j = 0; j < R::NF; ++j) {
-            float m = -INFINITY, s = 0.f;
+            const int n = n0 + R::col0(wn, j) + (lane & 15);
+            range[j] = listed_range<LIST>(s, min(n, rows - 1), m0, R::TILE_M);      // no branch around the loads: they go out together
+            if (n >= rows) range[j].y = range[j].x;
+        }
+#pragma unroll
+        for (int j = 0; j < R::NF; ++j) {
+            f32x4 v[R::MF];
+            hold<R>(acc, j);
+#pragma unroll
+            for (int i = 0; i < R::MF; ++i) {
+                v[i] = take(acc[i][j]);
+                if (m0 + R::TILE_M > vocab)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) v[i][r] = m0 + R::row0(wm, i) + g4 + r < vocab ? v[i][r] : -INFINITY;
+            }
+            float m = -INFINITY, sum = 0.f;
 #pragma unroll
             for (int i = 0; i < R::MF; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (m0 + R::row0(wm, i) + g4 + r >= vocab) acc[i][j][r] = -INFINITY;
-                    m = fmaxf(m, acc[i][j][r]);
-                }
+                for (int r = 0; r < 4; ++r) m = fmaxf(m, v[i][r]);
             m = fmaxf(m, __shfl_xor(m, 16));
             m = fmaxf(m, __shfl_xor(m, 32));
             const float at = m == -INFINITY ? 0.f : m;                   // no value above -inf: the sum is 0, not NaN
 #pragma unroll
             for (int i = 0; i < R::MF; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[i][j][r] - at) * c);
-            s += __shfl_xor(s, 16);
-            s += __shfl_xor(s, 32);
-            if (lane < 16) join[wm * R::TILE_N + R::col0(wn, j) + lane] = make_float2(m, s);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < R::NF; ++j) {
-            const int col = R::col0(wn, j) + (lane & 15), n = n0 + col;
-            const int2 at = range[col];
-            for (int e = at.x; e < at.y; ++e) {
-                const int want = ids[(int64_t)n * top + e] - m0 - g4;
-                float v = 0.f;
+                for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f((v[i][r] - at) * c);
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            if (lane < 16) join[wm * R::TILE_N + R::col0(wn, j) + lane] = make_float2(m, sum);
+            const int64_t row = (int64_t)(n0 + R::col0(wn, j) + (lane & 15)) * top;
+            for (int e = range[j].x; e < range[j].y; ++e) {
+                const int want = s.ids[row + e] - m0 - g4;
+                float z = 0.f;
                 bool mine = false;
 #pragma unroll
                 for (int i = 0; i < R::MF; ++i)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         if (want == R::row0(wm, i) + r) {
-                            v = acc[i][j][r];
+                            z = v[i][r];
                             mine = true;
                         }
-                if (mine) z[(int64_t)n * top + e] = v;
+                if (mine) s.z[row + e] = z;
             }
         }
+        lds_barrier();
         for (int i = tid; i < R::TILE_N; i += R::THREADS) {
             if (n0 + i >= rows) continue;
-            float m = -INFINITY, s = 0.f;
+            float m = -INFINITY, sum = 0.f;
 #pragma unroll
             for (int w = 0; w < R::WAVES_M; ++w) m = fmaxf(m, join[w * R::TILE_N + i].x);
             const float at = m == -INFINITY ? 0.f : m;
 #pragma unroll
             for (int w = 0; w < R::WAVES_M; ++w) {
                 const float2 v = join[w * R::TILE_N + i];
-                s += v.x == -INFINITY ? v.y : v.y * __builtin_amdgcn_exp2f((v.x - at) * c);
+                sum += v.x == -INFINITY ? v.y : v.y * __builtin_amdgcn_exp2f((v.x - at) * c);
             }
-            part[(int64_t)(n0 + i) * p.tiles_m + t.m] = make_float2(m, s);
+            part[(int64_t)(n0 + i) * p.tiles_m + t.m] = make_float2(m, sum);
         }
     }
 };
 
 // ---- backward: G = p - q of a piece of the vocabulary, and its transpose ----------------------------------------------------------
-template <int KIND>
+// The listed entries come from the z of the forward pass, p - q in fp32 before the one rounding.  Both matrices leave through LDS, 16 rows (fp32: 8)
+// of a wave's tile at a time, as whole lines and past the caches: see store_tile.
+template <int KIND, bool LIST>
 struct GradEpi {
     typedef typename Elem<KIND>::T T;
     T* g;              // [padded rows][pitch_g]
@@ -135,48 +141,95 @@ struct GradEpi {
     Saved s;
     int rows, from, size, top;     // this piece: ids from .. from + size
     float c;
-    bool listed_q;                 // distillation: q is in s.q; else 1
+    template <class R> static constexpr int wave_lds() {
+        constexpr int m = R::TILE_M / R::WAVES_M, n = R::TILE_N / R::WAVES_N;
+        return Stage<T, (m > n ? m : n)>::BYTES;
+    }
+    template <class R> static constexpr int lds() { return R::WAVES_M * R::WAVES_N * wave_lds<R>(); }
+    // staged rows of N elements -> memory
+    template <int N>
+    __device__ __forceinline__ static void put(const char* stage, T* to, int64_t pitch, int lane) {
+        typedef Stage<T, N> S;
+        struct alignas(16) Chunk { T v[16 / sizeof(T)]; };               // what was staged as T is read as T
+        wave_sync();
+#pragma unroll
+        for (int r = 0; r < S::ROWS; r += 64 / S::LANES) {
+            const int row = r + lane / S::LANES, at = (lane % S::LANES) * 16;
+            if (64 / S::LANES <= S::ROWS || row < S::ROWS) __builtin_nontemporal_store(__builtin_bit_cast(i32x4, *(const Chunk*)(stage + S::at(row, at))), (i32x4*)((char*)(to + row * pitch) + at));
+        }
+        wave_sync();
+    }
     template <class R>
     __device__ __forceinline__ void operator()(const Problem& p, Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF]) const {
-        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / R::WAVES_N, wn = wave % R::WAVES_N;
-        const int m0 = t.m * R::TILE_M, n0 = t.n * R::TILE_N, g4 = (lane >> 4) * 4;
+        constexpr int TM = R::TILE_M / R::WAVES_M, TN = R::TILE_N / R::WAVES_N;
+        const int tid = fresh(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / R::WAVES_N, wn = wave % R::WAVES_N;
+        const int m0 = t.m * R::TILE_M, n0 = t.n * R::TILE_N, g4 = (lane >> 4) * 4, col = lane & 15;
+        char* stage = lds + wave * wave_lds<R>();
+        struct alignas(4 * sizeof(T)) Four { T v[4]; };
+        hold<R>(acc, 0);
+        int2 range[R::NF];
+        int state[R::NF];
+        float2 norm[R::NF];
 #pragma unroll
         for (int j = 0; j < R::NF; ++j) {
-            const int n = n0 + R::col0(wn, j) + (lane & 15);
-            const int state = n < rows ? s.state[n] : ROW_SKIP;
-            const float2 norm = n < rows ? s.norm[n] : make_float2(0.f, 0.f);
-            const float inv = state == ROW_BAD ? __builtin_nanf("") : norm.y * Elem<KIND>::G_SCALE;
+            const int n = n0 + R::col0(wn, j) + col;
+            const int at = min(n, rows - 1);                             // no branch around the loads: they go out together
+            state[j] = s.state[at];
+            norm[j] = s.norm[at];
+            range[j] = listed_range<LIST>(s, at, from + m0, R::TILE_M);
+            if (n >= rows) state[j] = ROW_SKIP;
+        }
+        typedef Stage<T, TM> SG;
+        typedef Stage<T, TN> ST;
+        Four packed[R::MF][R::NF];                                       // 32-bit: as many registers as the sums took
+#pragma unroll
+        for (int j = 0; j < R::NF; ++j) {
+            f32x4 v[R::MF];
+            hold<R>(acc, j);
+            const float inv = state[j] == ROW_BAD ? __builtin_nanf("") : norm[j].y * Elem<KIND>::G_SCALE;
 #pragma unroll
             for (int i = 0; i < R::MF; ++i) {
-                const int m = m0 + R::row0(wm, i) + g4;
-                T v[4];
+                v[i] = take(acc[i][j]);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float e = __builtin_amdgcn_exp2f((acc[i][j][r] - norm.x) * c) * inv;
-                    v[r] = (T)(state == ROW_SKIP || m + r >= size ? 0.f : e);
+                    const float e = __builtin_amdgcn_exp2f((v[i][r] - norm[j].x) * c) * inv;
+                    v[i][r] = state[j] == ROW_SKIP || m0 + R::row0(wm, i) + g4 + r >= size ? 0.f : e;
                 }
-                struct alignas(4 * sizeof(T)) Four { T v[4]; };
-                *(Four*)(g + (int64_t)n * pitch_g + m) = Four{{v[0], v[1], v[2], v[3]}};
-                if (gt)
+            }
+            const int64_t row = (int64_t)(n0 + R::col0(wn, j) + col) * top;
+            if (state[j] == ROW_COUNT)
+                for (int e = range[j].x; e < range[j].y; ++e) {
+                    const int want = s.ids[row + e] - from - m0 - g4;
+                    const float q = LIST ? s.q[row + e] : 1.f;              // the cross entropy: 1
+                    const float d = (__builtin_amdgcn_exp2f((s.z[row + e] - norm[j].x) * c) * norm[j].y - q) * Elem<KIND>::G_SCALE;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) gt[(int64_t)(m + r) * pitch_gt + n] = v[r];
+                    for (int i = 0; i < R::MF; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) v[i][r] = want == R::row0(wm, i) + r ? d : v[i][r];
+                }
+            T* to = g + (int64_t)(n0 + R::col0(wn, j)) * pitch_g + m0 + R::row0(wm, 0);
+#pragma unroll
+            for (int i = 0; i < R::MF; ++i) packed[i][j] = Four{{(T)v[i][0], (T)v[i][1], (T)v[i][2], (T)v[i][3]}};
+#pragma unroll
+            for (int part = 0; part < 16; part += SG::ROWS) {
+#pragma unroll
+                for (int i = 0; i < R::MF; ++i)
+                    if (SG::ROWS == 16 || (col & ~(SG::ROWS - 1)) == part) *(Four*)(stage + SG::at(col & (SG::ROWS - 1), (i * 16 + g4) * (int)sizeof(T))) = packed[i][j];
+                put<TM>(stage, to + part * pitch_g, pitch_g, lane);
             }
         }
-        wait_loads<0>();                                                 // this wave's stores are done ...
-        barrier();                                                       // ... and everybody's: the listed entries go over them
-        for (int i = tid; i < R::TILE_N; i += R::THREADS) {
-            const int n = n0 + i;
-            if (n >= rows || s.state[n] != ROW_COUNT) continue;
-            const float2 norm = s.norm[n];
-            const int64_t row = (int64_t)n * top;
-            const int2 at = listed_range(s.ids + row, top, from + m0, R::TILE_M);
-            for (int e = at.x; e < at.y; ++e) {
-                const int m = s.ids[row + e] - from;
-                const float q = listed_q ? s.q[row + e] : 1.f;
-                const float v = __builtin_amdgcn_exp2f((s.z[row + e] - norm.x) * c) * norm.y - q;
-                const T out = (T)(v * Elem<KIND>::G_SCALE);
-                g[(int64_t)n * pitch_g + m] = out;
-                if (gt) gt[(int64_t)m * pitch_gt + n] = out;
+        if (!gt) return;
+#pragma unroll
+        for (int i = 0; i < R::MF; ++i) {
+            T* to = gt + (int64_t)(m0 + R::row0(wm, i)) * pitch_gt + n0 + R::col0(wn, 0);
+#pragma unroll
+            for (int part = 0; part < 16; part += ST::ROWS) {
+#pragma unroll
+                for (int j = 0; j < R::NF; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (ST::ROWS == 16 || (g4 & ~(ST::ROWS - 1)) == part) *(T*)(stage + ST::at((g4 + r) & (ST::ROWS - 1), (j * 16 + col) * (int)sizeof(T))) = packed[i][j].v[r];
+                put<TN>(stage, to + part * pitch_gt, pitch_gt, lane);
             }
         }
     }
@@ -187,28 +240,10 @@ struct SumEpi {
     float* out;        // [splits][rows][width]
     int rows, width;
     bool add;
+    template <class R> static constexpr int lds() { return stage_bytes<R, float>(); }
     template <class R>
     __device__ __forceinline__ void operator()(const Problem& p, Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF]) const {
-        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / R::WAVES_N, wn = wave % R::WAVES_N;
-        const int m0 = t.m * R::TILE_M, n0 = t.n * R::TILE_N, g4 = (lane >> 4) * 4;
-        const bool wide = (width & 3) == 0;
-#pragma unroll
-        for (int j = 0; j < R::NF; ++j) {
-            const int n = n0 + R::col0(wn, j) + (lane & 15);
-            if (n >= rows) continue;
-            float* to = out + ((int64_t)t.split * rows + n) * width;
-#pragma unroll
-            for (int i = 0; i < R::MF; ++i) {
-                const int m = m0 + R::row0(wm, i) + g4;
-                if (wide) {
-                    if (m < width) *(f32x4*)(to + m) = add ? *(const f32x4*)(to + m) + acc[i][j] : acc[i][j];
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (m + r < width) to[m + r] = add ? to[m + r] + acc[i][j][r] : acc[i][j][r];
-                }
-            }
-        }
+        store_tile<R>(t, lds, acc, out + (int64_t)t.split * rows * width, width, rows, width, add, [](float v) { return v; });
     }
 };
 
@@ -219,46 +254,20 @@ struct OutEpi {
     T* out;            // [rows of n][width]
     int rows, width;
     const float* scale;
+    template <class R> static constexpr int lds() { return stage_bytes<R, T>(); }
     template <class R>
     __device__ __forceinline__ void operator()(const Problem& p, Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF]) const {
-        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / R::WAVES_N, wn = wave % R::WAVES_N;
-        const int m0 = t.m * R::TILE_M, n0 = t.n * R::TILE_N, g4 = (lane >> 4) * 4;
-        const bool wide = (width & 3) == 0;
         const float f = *scale;
-        struct alignas(4 * sizeof(T)) Four { T v[4]; };
-#pragma unroll
-        for (int j = 0; j < R::NF; ++j) {
-            const int n = n0 + R::col0(wn, j) + (lane & 15);
-            if (n >= rows) continue;
-            T* to = out + (int64_t)n * width;
-#pragma unroll
-            for (int i = 0; i < R::MF; ++i) {
-                const int m = m0 + R::row0(wm, i) + g4;
-                T v[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = (T)(acc[i][j][r] * f);
-                if (wide) {
-                    if (m < width) *(Four*)(to + m) = Four{{v[0], v[1], v[2], v[3]}};
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (m + r < width) to[m + r] = v[r];
-                }
-            }
-        }
+        store_tile<R>(t, lds, acc, out, width, rows, width, false, [f](float v) { return v * f; });
     }
 };
 
 template <class R, class EPI>
 __global__ __launch_bounds__(R::THREADS) void product_kernel(Problem p, EPI epi) {
-    __shared__ __attribute__((aligned(1024))) char lds[R::LDS_BYTES];
-    const Tile t = tile_of(blockIdx.x, p);
-    f32x4 acc[R::MF][R::NF];
-    R::run(p, t, lds, acc);
-    epi.template operator()<R>(p, t, lds, acc);
+    __shared__ __attribute__((aligned(1024))) char lds[lds_bytes<R, EPI>()];
+    product<R>(p, lds, epi);
 }
 
-template <int KIND> using Large = Ring<KIND, 256, 256, 2, 4, 2>;
 template <int KIND> using Middle = Ring<KIND, 128, 128, 2, 2, 2>;
 template <int KIND> using Flat = Ring<KIND, 128, 32, 4, 1, 4>;
 
@@ -266,18 +275,19 @@ enum Shape { LARGE, MIDDLE, FLAT };
 struct ShapeSize { int m, n; };
 constexpr ShapeSize SHAPES[3] = {{256, 256}, {128, 128}, {128, 32}};
 
-Shape shape_for(int64_t m, int64_t n) {
+// splits: into how many runs of k the product may be cut
+Shape shape_for(int64_t m, int64_t n, int64_t splits = 1) {
     const int64_t large = ((m + 255) / 256) * ((n + 255) / 256);
     if (n <= 64) return FLAT;
-    return large >= 192 ? LARGE : MIDDLE;
+    return large * (splits > 1 ? splits : 1) >= 192 ? LARGE : MIDDLE;
 }
 
 struct Cut { int splits, per; };
-// k in so many runs that the tiles fill the 256 CUs about twice, of 4 slabs at least
+// k in so many runs that the tiles fill the 256 CUs (large tiles once, small ones twice), of 4 slabs at least
 Cut cut_for(int64_t m, int64_t n, int kbytes, Shape sh, int most) {
     const int64_t tiles = ((m + SHAPES[sh].m - 1) / SHAPES[sh].m) * ((n + SHAPES[sh].n - 1) / SHAPES[sh].n);
     const int slabs = (kbytes + 127) / 128;
-    int64_t splits = tiles >= 256 ? 1 : (512 + tiles - 1) / tiles;
+    int64_t splits = sh == LARGE ? (tiles >= 192 ? 1 : CUS / tiles) : tiles >= 256 ? 1 : (512 + tiles - 1) / tiles;
     if (splits > slabs / 4) splits = slabs / 4;
     if (splits > most) splits = most;
     if (splits < 1) splits = 1;
@@ -288,12 +298,11 @@ Cut cut_for(int64_t m, int64_t n, int kbytes, Shape sh, int most) {
 template <int KIND, class EPI>
 int launch_product(hipStream_t st, Shape sh, const Operand& a, const Operand& b, int kbytes, Cut cut, const EPI& epi) {
     Problem p{a, b, kbytes, nullptr, nullptr, 0, 0, (int)((a.rows + SHAPES[sh].m - 1) / SHAPES[sh].m), (int)((b.rows + SHAPES[sh].n - 1) / SHAPES[sh].n), cut.splits, cut.per};
-    const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n * p.splits;
-    CS_REQUIRE(blocks > 0 && blocks < (int64_t)1 << 31, "head loss: too many tiles");
-    const dim3 grid((unsigned)blocks);
-    if (sh == LARGE) product_kernel<Large<KIND>, EPI><<<grid, Large<KIND>::THREADS, 0, st>>>(p, epi);
-    else if (sh == MIDDLE) product_kernel<Middle<KIND>, EPI><<<grid, Middle<KIND>::THREADS, 0, st>>>(p, epi);
-    else product_kernel<Flat<KIND>, EPI><<<grid, Flat<KIND>::THREADS, 0, st>>>(p, epi);
+    CS_REQUIRE((int64_t)p.tiles_m * p.tiles_n * p.splits < (int64_t)1 << 31, "head loss: too many tiles");
+    if (sh == LARGE && p.kbytes % 128) product_kernel<Wide<KIND, true>, EPI><<<dim3(grid_of<Wide<KIND, true>>(p)), 256, 0, st>>>(p, epi);
+    else if (sh == LARGE) product_kernel<Wide<KIND, false>, EPI><<<dim3(grid_of<Wide<KIND, false>>(p)), 256, 0, st>>>(p, epi);
+    else if (sh == MIDDLE) product_kernel<Middle<KIND>, EPI><<<dim3(grid_of<Middle<KIND>>(p)), 256, 0, st>>>(p, epi);
+    else product_kernel<Flat<KIND>, EPI><<<dim3(grid_of<Flat<KIND>>(p)), 256, 0, st>>>(p, epi);
     CS_HIP(hipGetLastError());
     return CS_OK;
 }
@@ -415,6 +424,17 @@ __global__ __launch_bounds__(256) void teacher_rows_kernel(const void* ids, int 
         s.ids[to] = (int64_t)id < vocab ? (int)id : NO_ID;
         s.q[to] = q;
         s.z[to] = 0.f;
+    }
+    __syncthreads();
+    for (int64_t i = tid; i < s.starts_pitch; i += threads) {            // ids below 128 i among the ascending ones: a search of what was just written
+        const int64_t below = i * 128;
+        int lo = 0, hi = size;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if ((int64_t)(key[mid] >> 32) < below) lo = mid + 1;         // a place behind the last has id 2^32 - 1
+            else hi = mid;
+        }
+        s.starts[n * s.starts_pitch + i] = (uint16_t)(lo ? head[from][lo - 1] : 0);
     }
     for (int i = tid; i < top; i += threads)
         if (i >= used) {
@@ -591,14 +611,18 @@ Saved carve_saved(const cs_head_loss& h, void* base, size_t* bytes) {
     s.inv_count = a.take<float>(1);
     s.ids = a.take<int>(n * k);
     s.z = a.take<float>(n * k);
-    s.q = a.take<float>(h.kind == CS_HEAD_DISTILLATION ? n * k : 0);
+    const bool kd = h.kind == CS_HEAD_DISTILLATION;
+    s.q = a.take<float>(kd ? n * k : 0);
+    s.starts_pitch = (h.vocab + 255) / 256 * 2 + 1;
+    s.starts = a.take<uint16_t>(kd ? n * (size_t)s.starts_pitch : 0);
+    if (!kd) s.starts = nullptr;
     *bytes = a.at;
     return s;
 }
 
 // whether the product can read an operand where it lies
 bool in_place(const void* p, int64_t pitch, int64_t width, int size) {
-    return ((uintptr_t)p & 15) == 0 && (pitch * size) % 16 == 0 && (width * size) % 16 == 0 && pitch * size < ((int64_t)1 << 28);
+    return ((uintptr_t)p & 15) == 0 && (pitch * size) % 16 == 0 && (width * size) % 16 == 0 && pitch * size < ((int64_t)1 << 25);
 }
 
 struct Plan {
@@ -608,6 +632,9 @@ struct Plan {
     float2* part;
     double *losses, *entropy;
     int64_t padded, piece;                 // rows and vocabulary of a piece, rounded up to 256
+    // elements between the rows of G, W^T (piece_pitch), G^T and H^T (row_pitch): 128 bytes more than the rows, since rows a power of two apart
+    // meet in few memory channels (a product over 65 536-byte rows: 1100 instead of 1450 TFLOP/s)
+    int64_t piece_pitch, row_pitch;
     Cut cut;                               // of the sums of dH over the first piece; a shorter last piece adds to fewer of them
     Shape dh_shape;
     char *g, *gt, *wt, *ht;
@@ -636,19 +663,22 @@ Plan make_plan(const cs_head_loss& h, int backward, void* base) {
         p.piece = PIECE_BYTES / (p.padded * size) / 256 * 256;
         if (p.piece < 256) p.piece = 256;
         if (p.piece > up(h.vocab, 256)) p.piece = up(h.vocab, 256);
-        p.g = a.take<char>((size_t)(p.padded * p.piece * size));
+        p.piece_pitch = p.piece + 128 / size;
+        p.row_pitch = p.padded + 128 / size;
+        p.g = a.take<char>((size_t)(p.padded * p.piece_pitch * size));
         p.to_h = a.take<float>((size_t)h.rows);
         p.in_w = a.take<float>((size_t)h.rows);
         p.w_scale = a.take<float>(1);
         if (backward & 1) {
-            p.dh_shape = shape_for(h.width, h.rows);
-            p.cut = cut_for(h.width, h.rows, (int)((p.piece < h.vocab ? p.piece : up(h.vocab, 64)) * size), p.dh_shape, 64);
-            p.wt = a.take<char>((size_t)(h.width * p.piece * size));
+            const int kbytes = (int)((p.piece < h.vocab ? p.piece : up(h.vocab, 64)) * size);
+            p.dh_shape = shape_for(h.width, h.rows, kbytes / 128 / 32);  // runs of 32 slabs at least for large tiles
+            p.cut = cut_for(h.width, h.rows, kbytes, p.dh_shape, 64);
+            p.wt = a.take<char>((size_t)(h.width * p.piece_pitch * size));
             p.sums = a.take<float>((size_t)p.cut.splits * h.rows * h.width);
         }
         if (backward & 2) {
-            p.gt = a.take<char>((size_t)(p.padded * p.piece * size));
-            p.ht = a.take<char>((size_t)(h.width * p.padded * size));
+            p.gt = a.take<char>((size_t)(p.piece * p.row_pitch * size));
+            p.ht = a.take<char>((size_t)(h.width * p.row_pitch * size));
         }
     }
     p.bytes = a.at;
@@ -704,8 +734,10 @@ int forward(const cs_head_loss& h, const Plan& p, const Saved& s, float* row_los
         const float c = (float)(1.4426950408889634 / h.temperature);
         const Shape sh = shape_for(h.vocab, h.rows);
         const int tiles = (int)((h.vocab + SHAPES[sh].m - 1) / SHAPES[sh].m);
-        const NormEpi epi{p.part, s.z, s.ids, (int)h.rows, (int)h.vocab, h.top, c};
-        if (int rc = launch_product<KIND>(st, sh, a, b, kbytes, Cut{1, (kbytes + 127) / 128}, epi)) return rc;
+        const Cut whole{1, (kbytes + 127) / 128};
+        if (int rc = kd ? launch_product<KIND>(st, sh, a, b, kbytes, whole, NormEpi<true>{p.part, s, (int)h.rows, (int)h.vocab, h.top, c})
+                        : launch_product<KIND>(st, sh, a, b, kbytes, whole, NormEpi<false>{p.part, s, (int)h.rows, (int)h.vocab, h.top, c}))
+            return rc;
         row_loss_kernel<<<dim3((unsigned)((h.rows + 3) / 4)), 256, 0, st>>>(p.part, tiles, h.rows, h.top, kd, c, h.temperature, p.entropy, s, p.losses, row_losses);
     }
     reduce_loss_kernel<<<1, 1024, 0, st>>>(p.losses, s.state, h.rows, h.reduction == CS_REDUCE_MEAN, loss, s.inv_count);
@@ -729,24 +761,29 @@ int backward(const cs_head_loss& h, const Plan& p, const Saved& s, const float* 
     if (p.hidden) copy_rows<T>(st, h.hidden, h.hidden_pitch, h.rows, h.width, p.hidden, p.hidden_pitch);
     if (p.weight) copy_rows<T>(st, h.weight, h.weight_pitch, h.vocab, h.width, p.weight, p.weight_pitch);
     const int kbytes = (int)(p.hidden || p.weight ? up(h.width * size, 16) : h.width * size);
-    if (gw) transpose<T>(st, h.hidden, h.hidden_pitch, h.rows, h.width, p.ht, p.padded, up(h.rows, 32), p.in_w);
+    if (gw) transpose<T>(st, h.hidden, h.hidden_pitch, h.rows, h.width, p.ht, p.row_pitch, up(h.rows, 32), p.in_w);
     for (int64_t from = 0; from < h.vocab; from += p.piece) {
         const int64_t len = h.vocab - from < p.piece ? h.vocab - from : p.piece, klen = up(len, 64);
         const Operand a{(p.weight ? p.weight : (const char*)h.weight) + from * p.weight_pitch, p.weight_pitch, len};
         const Operand b{p.hidden ? p.hidden : (const char*)h.hidden, p.hidden_pitch, h.rows};
-        const GradEpi<KIND> grad_epi{(T*)p.g, gw ? (T*)p.gt : nullptr, p.piece, p.padded, s, (int)h.rows, (int)from, (int)len, h.top, c, kd};
-        if (int rc = launch_product<KIND>(st, shape_for(len, h.rows), a, b, kbytes, Cut{1, (kbytes + 127) / 128}, grad_epi)) return rc;
+        const Cut whole{1, (kbytes + 127) / 128};
+        T* const g = (T*)p.g;
+        T* const gt = gw ? (T*)p.gt : nullptr;
+        const Shape sh = shape_for(len, h.rows);
+        if (int rc = kd ? launch_product<KIND>(st, sh, a, b, kbytes, whole, GradEpi<KIND, true>{g, gt, p.piece_pitch, p.row_pitch, s, (int)h.rows, (int)from, (int)len, h.top, c})
+                        : launch_product<KIND>(st, sh, a, b, kbytes, whole, GradEpi<KIND, false>{g, gt, p.piece_pitch, p.row_pitch, s, (int)h.rows, (int)from, (int)len, h.top, c}))
+            return rc;
         if (gh) {
-            transpose<T>(st, (const T*)h.weight + from * h.weight_pitch, h.weight_pitch, len, h.width, p.wt, p.piece, klen, nullptr);
+            transpose<T>(st, (const T*)h.weight + from * h.weight_pitch, h.weight_pitch, len, h.width, p.wt, p.piece_pitch, klen, nullptr);
             const int kb = (int)(klen * size), slabs = (kb + 127) / 128;
             const Cut cut{(slabs + p.cut.per - 1) / p.cut.per, p.cut.per};
             const SumEpi epi{p.sums, (int)h.rows, (int)h.width, from != 0};
-            if (int rc = launch_product<KIND>(st, p.dh_shape, Operand{p.wt, p.piece * size, h.width}, Operand{p.g, p.piece * size, h.rows}, kb, cut, epi)) return rc;
+            if (int rc = launch_product<KIND>(st, p.dh_shape, Operand{p.wt, p.piece_pitch * size, h.width}, Operand{p.g, p.piece_pitch * size, h.rows}, kb, cut, epi)) return rc;
         }
         if (gw) {
             const int kb = (int)(up(h.rows, 32) * size);
             const OutEpi<KIND> epi{(T*)gw + from * h.width, (int)len, (int)h.width, p.w_scale};
-            if (int rc = launch_product<KIND>(st, shape_for(h.width, len), Operand{p.ht, p.padded * size, h.width}, Operand{p.gt, p.padded * size, len}, kb,
+            if (int rc = launch_product<KIND>(st, shape_for(h.width, len), Operand{p.ht, p.row_pitch * size, h.width}, Operand{p.gt, p.row_pitch * size, len}, kb,
                                               Cut{1, (kb + 127) / 128}, epi))
                 return rc;
         }

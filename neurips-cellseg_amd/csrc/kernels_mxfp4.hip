@@ -124,45 +124,19 @@ template <class T>
 struct LinearEpi {
     T* out;            // [rows][outputs]
     int rows, outputs;
+    template <class R> static constexpr int lds() { return stage_bytes<R, T>(); }
     template <class R>
     __device__ __forceinline__ void operator()(const Problem& p, Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF]) const {
-        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / R::WAVES_N, wn = wave % R::WAVES_N;
-        const int m0 = t.m * R::TILE_M, n0 = t.n * R::TILE_N, g4 = (lane >> 4) * 4;
-        const bool wide = (outputs & 3) == 0;
-        struct alignas(4 * sizeof(T)) Four { T v[4]; };
-#pragma unroll
-        for (int j = 0; j < R::NF; ++j) {
-            const int n = n0 + R::col0(wn, j) + (lane & 15);
-            if (n >= rows) continue;
-            T* to = out + (int64_t)n * outputs;
-#pragma unroll
-            for (int i = 0; i < R::MF; ++i) {
-                const int m = m0 + R::row0(wm, i) + g4;
-                T v[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = (T)acc[i][j][r];
-                if (wide) {
-                    if (m < outputs) *(Four*)(to + m) = Four{{v[0], v[1], v[2], v[3]}};
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (m + r < outputs) to[m + r] = v[r];
-                }
-            }
-        }
+        store_tile<R>(t, lds, acc, out, outputs, rows, outputs, false, [](float v) { return v; });
     }
 };
 
 template <class R, class EPI>
 __global__ __launch_bounds__(R::THREADS) void linear_kernel(Problem p, EPI epi) {
-    __shared__ __attribute__((aligned(1024))) char lds[R::LDS_BYTES];
-    const Tile t = tile_of(blockIdx.x, p);
-    f32x4 acc[R::MF][R::NF];
-    R::run(p, t, lds, acc);
-    epi.template operator()<R>(p, t, lds, acc);
+    __shared__ __attribute__((aligned(1024))) char lds[lds_bytes<R, EPI>()];
+    product<R>(p, lds, epi);
 }
 
-typedef Ring<E2M1, 256, 256, 2, 4, 2> Large;
 typedef Ring<E2M1, 128, 128, 2, 2, 2> Middle;
 typedef Ring<E2M1, 128, 32, 4, 1, 4> Flat;
 
@@ -172,9 +146,8 @@ int launch_linear(hipStream_t st, Problem p, LinearEpi<T> epi) {
     p.tiles_n = (int)((p.b.rows + R::TILE_N - 1) / R::TILE_N);
     p.splits = 1;
     p.slabs_per_split = (p.kbytes + 127) / 128;
-    const int64_t blocks = (int64_t)p.tiles_m * p.tiles_n;
-    CS_REQUIRE(blocks < (int64_t)1 << 31, "mxfp4 linear: too many tiles");
-    linear_kernel<R, LinearEpi<T>><<<dim3((unsigned)blocks), R::THREADS, 0, st>>>(p, epi);
+    CS_REQUIRE((int64_t)p.tiles_m * p.tiles_n < (int64_t)1 << 31, "mxfp4 linear: too many tiles");
+    linear_kernel<R, LinearEpi<T>><<<dim3(grid_of<R>(p)), R::THREADS, 0, st>>>(p, epi);
     CS_HIP(hipGetLastError());
     return CS_OK;
 }
@@ -251,7 +224,11 @@ int linear(const void* x, int64_t pitch, int64_t rows, int64_t width, const uint
     q.rows_b = p.rows_x;
     const LinearEpi<T> epi{(T*)y, (int)rows, (int)outputs};
     if (rows <= 64) return launch_linear<Flat>(st, q, epi);
-    if (((outputs + 255) / 256) * ((rows + 255) / 256) >= 192) return launch_linear<Large>(st, q, epi);
+    if (((outputs + 255) / 256) * ((rows + 255) / 256) >= 192) {
+        // whole pairs of slabs, or zeros behind the end
+        if (q.kbytes % 256) return launch_linear<Wide<E2M1, true>>(st, q, epi);
+        return launch_linear<Wide<E2M1, false>>(st, q, epi);
+    }
     return launch_linear<Middle>(st, q, epi);
 }
 

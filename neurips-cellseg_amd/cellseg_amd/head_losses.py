@@ -34,7 +34,8 @@ def _pitch(t: torch.Tensor) -> int:
 
 def rows_of(t: torch.Tensor) -> torch.Tensor:
     """[..., D] -> [rows, D] with unit inner stride and rows that do not overlap; a copy only where the strides do not allow a view."""
-    t = t.reshape(-1, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
     if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
         t = t.contiguous()
     return t
@@ -50,9 +51,10 @@ def _checked(hidden: torch.Tensor, weight: torch.Tensor, reduction: str, ids: to
     if ids.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"{name} holds int64 or int32, got {ids.dtype}")
     for t in (hidden, weight, ids):
-        _lib.require_gpu(t)
-        if t.device != hidden.device:
-            raise ValueError(f"hidden, weight and {name} are on one device, got {hidden.device} and {t.device}")
+        if not t.is_cuda:
+            _lib.require_gpu(t)
+    if weight.device != hidden.device or ids.device != hidden.device:
+        raise ValueError(f"hidden, weight and {name} are on one device, got {hidden.device}, {weight.device} and {ids.device}")
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *, ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
@@ -63,7 +65,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     _checked(hidden, weight, reduction, target, "target")
     if target.shape != hidden.shape[:-1]:
         raise ValueError(f"expected target {tuple(hidden.shape[:-1])}, got {tuple(target.shape)}")
-    losses = _HeadLoss.apply(rows_of(hidden), rows_of(weight), target.reshape(-1), None, _CROSS_ENTROPY, _REDUCTIONS[reduction], int(ignore_index), 1.0)
+    losses = _HeadLoss.apply(rows_of(hidden), rows_of(weight), target if target.dim() == 1 else target.reshape(-1), None, _CROSS_ENTROPY, _REDUCTIONS[reduction], int(ignore_index), 1.0)
     return losses.reshape(target.shape) if reduction == "none" else losses
 
 
@@ -135,31 +137,33 @@ class _HeadLoss(torch.autograd.Function):
         top = 1 if teacher is None else ids.shape[1]
         head = _descriptor(hidden, weight, kind, reduction, ignore_index, temperature, top, ids, teacher)
         with torch.cuda.device(hidden.device):
-            size = int(lib.cs_head_loss_saved_bytes(C.byref(head)))
+            size = lib.cs_head_loss_saved_bytes(head)
             if not size:
                 check(-1, "cs_head_loss_saved_bytes")
             saved = torch.empty(size, dtype=torch.uint8, device=hidden.device)
-            ws = torch.empty(max(1, int(lib.cs_head_loss_workspace_bytes(C.byref(head), 0))), dtype=torch.uint8, device=hidden.device)
+            ws = torch.empty(lib.cs_head_loss_workspace_bytes(head, 0) or 1, dtype=torch.uint8, device=hidden.device)
             loss = torch.empty((hidden.shape[0],) if reduction == 0 else (), dtype=torch.float32, device=hidden.device)
-            to = C.c_void_p(loss.data_ptr())
-            check(lib.cs_head_loss_forward(C.byref(head), to if reduction == 0 else None, None if reduction == 0 else to, C.c_void_p(saved.data_ptr()), saved.numel(),
-                                           C.c_void_p(ws.data_ptr()), ws.numel(), _lib.stream_ptr()), "cs_head_loss_forward")
+            to = loss.data_ptr()
+            check(lib.cs_head_loss_forward(head, to if reduction == 0 else None, None if reduction == 0 else to, saved.data_ptr(), saved.numel(), ws.data_ptr(), ws.numel(),
+                                           _lib.stream_ptr()), "cs_head_loss_forward")
         ctx.save_for_backward(hidden, weight, saved)
-        ctx.cfg = (kind, reduction, ignore_index, temperature, top)
+        ctx.head = head
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         hidden, weight, saved = ctx.saved_tensors
-        head = _descriptor(hidden, weight, *ctx.cfg)
-        want = (1 if ctx.needs_input_grad[0] else 0) | (2 if ctx.needs_input_grad[1] else 0)
-        grad = grad.float()
+        head = ctx.head
+        head.hidden, head.weight = hidden.data_ptr(), weight.data_ptr()      # a saved-tensor hook may have moved them, with new strides
+        head.hidden_pitch, head.weight_pitch = _pitch(hidden), _pitch(weight)
+        need = ctx.needs_input_grad
+        if grad.dtype != torch.float32:
+            grad = grad.float()
         with torch.cuda.device(hidden.device):
-            ws = torch.empty(max(1, int(lib.cs_head_loss_workspace_bytes(C.byref(head), want))), dtype=torch.uint8, device=hidden.device)
-            gh = torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device) if want & 1 else None
-            gw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if want & 2 else None
-            check(lib.cs_head_loss_backward(C.byref(head), C.c_void_p(saved.data_ptr()), saved.numel(), C.c_void_p(grad.data_ptr()), grad.stride(0) if grad.dim() else 0,
-                                            C.c_void_p(gh.data_ptr()) if want & 1 else None, C.c_void_p(gw.data_ptr()) if want & 2 else None,
-                                            C.c_void_p(ws.data_ptr()), ws.numel(), _lib.stream_ptr()), "cs_head_loss_backward")
+            gh = torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device) if need[0] else None
+            gw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if need[1] else None
+            ws = torch.empty(lib.cs_head_loss_workspace_bytes(head, need[0] + 2 * need[1]) or 1, dtype=torch.uint8, device=hidden.device)
+            check(lib.cs_head_loss_backward(head, saved.data_ptr(), saved.numel(), grad.data_ptr(), grad.stride(0) if grad.dim() else 0, gh.data_ptr() if need[0] else None,
+                                            gw.data_ptr() if need[1] else None, ws.data_ptr(), ws.numel(), _lib.stream_ptr()), "cs_head_loss_backward")
         return gh, gw, None, None, None, None, None, None

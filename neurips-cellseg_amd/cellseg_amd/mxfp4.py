@@ -6,7 +6,6 @@ sums (csrc/kernels_mxfp4.hip).  For serving: no gradients.
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import Optional, Tuple
 
 import torch
@@ -52,8 +51,8 @@ class MXFP4Tensor:
         _lib.require_gpu(self.codes)
         out = torch.empty(self.shape, dtype=dtype, device=self.device)
         with torch.cuda.device(self.device):
-            check(lib.cs_mxfp4_dequantize(C.c_void_p(self.codes.data_ptr()), C.c_void_p(self.scales.data_ptr()), out.numel() // self.width, self.width, TYPES[dtype],
-                                          C.c_void_p(out.data_ptr()), _lib.stream_ptr()), "cs_mxfp4_dequantize")
+            check(lib.cs_mxfp4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), out.numel() // self.width, self.width, TYPES[dtype],
+                                          out.data_ptr(), _lib.stream_ptr()), "cs_mxfp4_dequantize")
         return out
 
     def __repr__(self) -> str:
@@ -78,8 +77,8 @@ def mxfp4_quantize(x: torch.Tensor) -> MXFP4Tensor:
     codes = torch.empty(tuple(x.shape[:-1]) + (16 * blocks,), dtype=torch.uint8, device=x.device)
     scales = torch.empty(tuple(x.shape[:-1]) + (blocks,), dtype=torch.uint8, device=x.device)
     with torch.cuda.device(x.device):
-        check(lib.cs_mxfp4_quantize(C.c_void_p(rows.data_ptr()), _pitch(rows), rows.shape[0], width, TYPES[x.dtype], C.c_void_p(codes.data_ptr()),
-                                    C.c_void_p(scales.data_ptr()), _lib.stream_ptr()), "cs_mxfp4_quantize")
+        check(lib.cs_mxfp4_quantize(rows.data_ptr(), _pitch(rows), rows.shape[0], width, TYPES[x.dtype], codes.data_ptr(),
+                                    scales.data_ptr(), _lib.stream_ptr()), "cs_mxfp4_quantize")
     return MXFP4Tensor(codes, scales, width, x.dtype)
 
 
@@ -92,15 +91,14 @@ def mxfp4_linear(x: torch.Tensor, weight: MXFP4Tensor) -> torch.Tensor:
         raise TypeError(f"mxfp4_linear takes bfloat16, float16 or float32, got {x.dtype}")
     if x.dim() < 1 or len(weight.shape) != 2 or x.shape[-1] != weight.width:
         raise ValueError(f"expected x [..., {weight.width}] and weight [outputs, {weight.width}], got {tuple(x.shape)} and {weight.shape}")
-    _lib.require_gpu(x)
+    if not x.is_cuda:
+        _lib.require_gpu(x)
     if weight.device != x.device:
         raise ValueError(f"weight is on {weight.device}, x on {x.device}")
     rows, outputs = rows_of(x), weight.shape[0]
     y = torch.empty(tuple(x.shape[:-1]) + (outputs,), dtype=x.dtype, device=x.device)
     with torch.cuda.device(x.device):
-        size = int(lib.cs_mxfp4_linear_workspace_bytes(rows.shape[0], weight.width, outputs))
-        ws = torch.empty(max(1, size), dtype=torch.uint8, device=x.device)
-        check(lib.cs_mxfp4_linear(C.c_void_p(rows.data_ptr()), _pitch(rows), rows.shape[0], weight.width, TYPES[x.dtype], C.c_void_p(weight.codes.data_ptr()),
-                                  C.c_void_p(weight.scales.data_ptr()), outputs, C.c_void_p(y.data_ptr()), C.c_void_p(ws.data_ptr()), ws.numel(), _lib.stream_ptr()),
-              "cs_mxfp4_linear")
+        ws = torch.empty(lib.cs_mxfp4_linear_workspace_bytes(rows.shape[0], weight.width, outputs) or 1, dtype=torch.uint8, device=x.device)
+        check(lib.cs_mxfp4_linear(rows.data_ptr(), _pitch(rows), rows.shape[0], weight.width, TYPES[x.dtype], weight.codes.data_ptr(), weight.scales.data_ptr(), outputs,
+                                  y.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_ptr()), "cs_mxfp4_linear")
     return y

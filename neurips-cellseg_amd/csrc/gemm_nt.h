@@ -357,7 +357,7 @@ struct Wide {
                 before(n);
                 __builtin_amdgcn_sched_barrier(0);
                 each<PER>([&](auto q) {
-                    constexpr int N = n.value * PER + q.value, E = N >> 6, I = (N & 63) >> 3, J = N & 7;
+                    constexpr int N = n.value * PER + q.value, E = N >> 6, I = (N & 63) >> 3, J = I & 1 ? 7 - (N & 7) : N & 7;
                     mma_in_place<KIND, 2 * odd.value + h.value>(acc[I][J], a[h.value][I], b[h.value][J], E, scale[NF + I], scale[J]);
                 });
                 __builtin_amdgcn_sched_barrier(0);

@@ -544,27 +544,46 @@ __global__ __launch_bounds__(1024) void row_scale_kernel(const float* grad, int6
     if (tid == 0) *w_scale = (per_row ? (big == 0.f ? 1.f : big) : one) * f;
 }
 
-// src [rows][cols] (element pitch) -> dst [cols][pitch], columns of dst behind the rows zero up to `padded`; row n times scale[n] (NULL: 1; 0 selects 0)
+// src [rows][cols] (element pitch) -> dst [cols][pitch], columns of dst behind the rows zero up to `padded`; row n times scale[n] (NULL: 1; 0 selects 0).
+// 16 bytes a lane on both sides; the tile of 8 x 8 chunks lies in LDS with chunk c of row r at c ^ (r / E), so that a column is read from all banks.
 template <class T>
 __global__ __launch_bounds__(256) void transpose_kernel(const T* src, int64_t src_pitch, int64_t rows, int64_t cols, T* dst, int64_t dst_pitch, int64_t padded,
-                                                        const float* scale) {
-    __shared__ T tile[64][64 + 4 / sizeof(T) + 1];
-    const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
-    const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-    for (int i = y; i < 64; i += 4) {
-        T v = (T)0.f;
-        if (r0 + i < rows && c0 + x < cols) {
-            v = src[(r0 + i) * src_pitch + c0 + x];
+                                                        const float* scale, bool wide) {
+    constexpr int E = 16 / (int)sizeof(T), SIDE = 8 * E, CHUNKS = SIDE * 8;
+    struct alignas(16) Chunk { T v[E]; };
+    __shared__ Chunk tile[CHUNKS];
+    const int64_t r0 = (int64_t)blockIdx.x * SIDE, c0 = (int64_t)blockIdx.y * SIDE;
+#pragma unroll
+    for (int i = threadIdx.x; i < CHUNKS; i += 256) {
+        const int r = i >> 3, ch = i & 7;
+        const int64_t row = r0 + r, col = c0 + ch * E;
+        Chunk v{};
+        if (row < rows && col < cols) {
+            const T* from = src + row * src_pitch + col;
+            if (wide && col + E <= cols) v = *(const Chunk*)from;
+            else
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (col + e < cols) v.v[e] = from[e];
             if (scale) {
-                const float f = scale[r0 + i];
-                v = f == 0.f ? (T)0.f : f == 1.f ? v : (T)((float)v * f);
+                const float f = scale[row];
+                if (f != 1.f)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) v.v[e] = f == 0.f ? (T)0.f : (T)((float)v.v[e] * f);
             }
         }
-        tile[i][x] = v;
+        tile[r * 8 + (ch ^ (r / E))] = v;
     }
     __syncthreads();
-    for (int i = y; i < 64; i += 4)
-        if (c0 + i < cols && r0 + x < padded) dst[(c0 + i) * dst_pitch + r0 + x] = tile[x][i];
+#pragma unroll
+    for (int i = threadIdx.x; i < CHUNKS; i += 256) {
+        const int c = i >> 3, ch = i & 7;                                // column c, rows ch * E ..
+        const int64_t col = c0 + c, row = r0 + ch * E;
+        Chunk v;
+#pragma unroll
+        for (int e = 0; e < E; ++e) v.v[e] = tile[(ch * E + e) * 8 + ((c / E) ^ ch)].v[c % E];
+        if (col < cols && row < padded) *(Chunk*)(dst + col * dst_pitch + row) = v;
+    }
 }
 
 // src [rows][cols] -> dst [rows][pitch], zeros behind the columns
@@ -573,10 +592,23 @@ __global__ __launch_bounds__(256) void copy_rows_kernel(const T* src, int64_t sr
     for (int64_t c = threadIdx.x; c < pitch; c += 256) dst[(int64_t)blockIdx.x * pitch + c] = c < cols ? src[(int64_t)blockIdx.x * src_pitch + c] : (T)0.f;
 }
 
+// the sums of all runs of k, in their order, times the row's factor; 4 columns a lane where rows are multiples of 4
 template <class T>
 __global__ __launch_bounds__(256) void hidden_grad_kernel(const float* sums, int splits, int64_t rows, int64_t width, const float* scale, T* out) {
     const int64_t n = blockIdx.x;
     const float f = scale[n];
+    if ((width & 3) == 0) {
+        struct alignas(4 * sizeof(T)) Four { T v[4]; };
+        for (int64_t c = (int64_t)threadIdx.x * 4; c < width; c += 1024) {
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+            for (int s = 0; s < splits; ++s) v += *(const f32x4*)(sums + ((int64_t)s * rows + n) * width + c);
+            Four to;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to.v[e] = (T)(f == 0.f ? 0.f : v[e] * f);
+            *(Four*)(out + n * width + c) = to;
+        }
+        return;
+    }
     for (int64_t c = threadIdx.x; c < width; c += 256) {
         float v = 0.f;
         for (int s = 0; s < splits; ++s) v += sums[((int64_t)s * rows + n) * width + c];
@@ -691,7 +723,10 @@ void copy_rows(hipStream_t st, const void* src, int64_t pitch, int64_t rows, int
 }
 template <class T>
 void transpose(hipStream_t st, const void* src, int64_t pitch, int64_t rows, int64_t cols, void* dst, int64_t dst_pitch, int64_t padded, const float* scale) {
-    transpose_kernel<T><<<dim3((unsigned)((padded + 63) / 64), (unsigned)((cols + 63) / 64)), 256, 0, st>>>((const T*)src, pitch, rows, cols, (T*)dst, dst_pitch, padded, scale);
+    constexpr int SIDE = 128 / (int)sizeof(T);
+    const bool wide = ((uintptr_t)src & 15) == 0 && pitch * (int64_t)sizeof(T) % 16 == 0;
+    transpose_kernel<T><<<dim3((unsigned)((padded + SIDE - 1) / SIDE), (unsigned)((cols + SIDE - 1) / SIDE)), 256, 0, st>>>((const T*)src, pitch, rows, cols, (T*)dst, dst_pitch,
+                                                                                                                           padded, scale, wide);
 }
 
 int check_head(const cs_head_loss* h) {

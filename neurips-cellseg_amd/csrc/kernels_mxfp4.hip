@@ -58,40 +58,54 @@ __device__ __forceinline__ int64_t tile_place(int64_t row, int64_t block, int64_
     return (((block >> 4) * rows + row) * 4 + (block & 3)) * 4 + ((block >> 2) & 3);
 }
 
-// 4 lanes a block.  TILED: scales in the product's order over `rows_tiled` rows, blocks up to a multiple of 16 and rows behind the last with
-// scale 1 and no codes; else [rows][blocks]
-template <class T, bool TILED>
-__global__ __launch_bounds__(256) void quantise_kernel(const T* x, int64_t pitch, int64_t rows, int64_t width, int64_t blocks, bool wide, uint8_t* codes, uint8_t* scales,
-                                                       int64_t rows_tiled) {
-    const int64_t per = TILED ? (blocks + 15) / 16 * 16 : blocks, total = (TILED ? rows_tiled : rows) * per * 4;
+// one block of 32 by 4 lanes: item i of rows x blocks x 4
+template <class T>
+__global__ __launch_bounds__(256) void quantise_kernel(const T* x, int64_t pitch, int64_t rows, int64_t width, int64_t blocks, bool wide, uint8_t* codes, uint8_t* scales) {
+    const int64_t total = rows * blocks * 4;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t b = i >> 2, row = b / per, block = b - row * per;
-        const int part = (int)(i & 3);
-        const bool in = !TILED || (row < rows && block < blocks);
+        const int64_t b = i >> 2, row = b / blocks, block = b - row * blocks;
         float v[8];
-        if (in) load8(x + row * pitch, block * 32 + part * 8, width, wide, v);
-        else
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = 0.f;
+        load8(x + row * pitch, block * 32 + (i & 3) * 8, width, wide, v);
         unsigned scale;
-        const unsigned code = encode8(v, &scale);
-        if (in) *(unsigned*)(codes + (row * blocks + block) * 16 + part * 4) = code;
-        if (part == 0) scales[TILED ? tile_place(row, block, rows_tiled) : row * blocks + block] = (uint8_t)(in ? scale : 127u);
+        *(unsigned*)(codes + i * 4) = encode8(v, &scale);
+        if ((i & 3) == 0) scales[b] = (uint8_t)scale;
     }
 }
 
-// [rows][blocks] scales -> the product's order
-__global__ __launch_bounds__(256) void tile_scales_kernel(const uint8_t* scales, int64_t rows, int64_t blocks, uint8_t* out, int64_t rows_tiled) {
-    const int64_t total = rows_tiled * ((blocks + 15) / 16) * 4;         // words of 4 blocks: 4 h' + g, h' = 0..3
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t g = i & 3, row = (i >> 2) % rows_tiled, pair = (i >> 2) / rows_tiled;
+// What the product reads: x quantised, and both operands' scales in its order (gemm_nt.h) over rows_x / rows_w rows, blocks up to a multiple of
+// 16, with scale 1 where there is no row or block.  The first `x_blocks` thread blocks take x, the others the weight's scales.
+template <class T>
+__global__ __launch_bounds__(256) void prepare_kernel(const T* x, int64_t pitch, int64_t rows, int64_t width, int64_t blocks, bool wide, uint8_t* codes, uint8_t* scales_x,
+                                                      int64_t rows_x, const uint8_t* scales, int64_t outputs, uint8_t* scales_w, int64_t rows_w, int x_blocks) {
+    const int64_t padded = (blocks + 15) / 16 * 16;
+    if ((int)blockIdx.x < x_blocks) {
+        const int64_t total = rows_x * padded * 4;
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)x_blocks * 256) {
+            const int64_t b = i >> 2, row = b / padded, block = b - row * padded;
+            const int part = (int)(i & 3);
+            const bool in = row < rows && block < blocks;                // the same in a block's 4 lanes
+            float v[8];
+            if (in) load8(x + row * pitch, block * 32 + part * 8, width, wide, v);
+            else
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = 0.f;
+            unsigned scale;
+            const unsigned code = encode8(v, &scale);
+            if (in) *(unsigned*)(codes + (row * blocks + block) * 16 + part * 4) = code;
+            if (part == 0) scales_x[tile_place(row, block, rows_x)] = (uint8_t)(in ? scale : 127u);
+        }
+        return;
+    }
+    const int64_t total = rows_w * (padded / 16) * 4;                    // words of 4 blocks: 4 h + g, h = 0..3
+    for (int64_t i = (int64_t)(blockIdx.x - x_blocks) * 256 + threadIdx.x; i < total; i += (int64_t)(gridDim.x - x_blocks) * 256) {
+        const int64_t g = i & 3, row = (i >> 2) % rows_w, pair = (i >> 2) / rows_w;
         unsigned word = 0;
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
             const int64_t block = pair * 16 + h * 4 + g;
-            word |= (row < rows && block < blocks ? (unsigned)scales[row * blocks + block] : 127u) << (8 * h);
+            word |= (row < outputs && block < blocks ? (unsigned)scales[row * blocks + block] : 127u) << (8 * h);
         }
-        ((unsigned*)out)[i] = word;
+        ((unsigned*)scales_w)[i] = word;
     }
 }
 
@@ -139,6 +153,60 @@ __global__ __launch_bounds__(R::THREADS) void linear_kernel(Problem p, EPI epi) 
 
 typedef Ring<E2M1, 128, 128, 2, 2, 2> Middle;
 typedef Ring<E2M1, 128, 32, 4, 1, 4> Flat;
+
+// Up to 16 rows, as a server decodes: the weights are read once and nothing else counts.  A block has 16 outputs; its 4 waves take runs of 8 blocks
+// of k (128 bytes of a weight row) in turn, straight from memory into the matrix instruction, and join their sums in LDS.  Every thread block
+// quantises the few rows for itself, into LDS: one launch instead of three, and x is in L2.
+constexpr int FEW_LDS = 40 << 10;                 // 4 blocks a CU
+__host__ __device__ inline int few_pitch(int blocks) { return (blocks + 3) / 4 * 64 + 16; }      // bytes of a row's codes, off the powers of two
+int few_lds(int64_t rows, int64_t blocks) { return blocks > 4096 ? FEW_LDS + 1 : (int)(rows * (few_pitch((int)blocks) + (blocks + 3) / 4 * 4)); }
+
+template <class T>
+__global__ __launch_bounds__(256) void few_rows_kernel(const T* x, int64_t pitch, int rows, int64_t width, int blocks, bool wide, const uint8_t* codes, const uint8_t* scales,
+                                                       int outputs, T* y) {
+    extern __shared__ __attribute__((aligned(16))) char few[];
+    __shared__ f32x4 join[4][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, steps = (blocks + 3) >> 2, cp = few_pitch(blocks), sp = steps * 4;
+    char* const xs = few + rows * cp;                                    // scales of x [rows][sp]
+    for (int i = tid; i < rows * sp * 4; i += 256) {
+        const int b = i >> 2, row = b / sp, block = b - row * sp;
+        float v[8];
+        load8(x + row * pitch, (int64_t)block * 32 + (i & 3) * 8, width, wide, v);   // zeros behind the width
+        unsigned scale;
+        *(unsigned*)(few + row * cp + block * 16 + (i & 3) * 4) = encode8(v, &scale);
+        if ((i & 3) == 0) xs[row * sp + block] = (char)scale;
+    }
+    __syncthreads();
+    const int g = lane >> 4, m0 = blockIdx.x * 16, m = min(m0 + (lane & 15), outputs - 1), n = (lane & 15) < rows ? lane & 15 : 0;
+    const uint8_t* wc = codes + (int64_t)m * blocks * 16;
+    const uint8_t* ws = scales + (int64_t)m * blocks;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int u = wave; 2 * u < steps; u += 4)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int step = 2 * u + h, block = step * 4 + g;
+            const bool in = block < blocks;
+            i32x4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+            int sa = 127, sb = 127;
+            if (in) {
+                a = *(const i32x4*)(wc + (int64_t)block * 16);
+                sa = ws[block];
+                b = *(const i32x4*)(few + n * cp + block * 16);
+                sb = (uint8_t)xs[n * sp + block];
+            }
+            acc = mma<E2M1, 0>(a, b, acc, sa, sb);
+        }
+    join[wave][lane] = acc;
+    __syncthreads();
+    if (wave == 0 && (lane & 15) < rows) {
+        acc = (join[0][lane] + join[1][lane]) + (join[2][lane] + join[3][lane]);
+        T* to = y + (int64_t)(lane & 15) * outputs;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (m0 + g * 4 + r < outputs) to[m0 + g * 4 + r] = (T)acc[r];
+    }
+}
 
 template <class R, class T>
 int launch_linear(hipStream_t st, Problem p, LinearEpi<T> epi) {
@@ -196,7 +264,7 @@ bool reads_wide(const void* x, int64_t pitch) {
 template <class T>
 int quantise(const void* x, int64_t pitch, int64_t rows, int64_t width, uint8_t* codes, uint8_t* scales, hipStream_t st) {
     const int64_t blocks = (width + 31) / 32;
-    quantise_kernel<T, false><<<grid_for(rows * blocks * 4), 256, 0, st>>>((const T*)x, pitch, rows, width, blocks, reads_wide<T>(x, pitch), codes, scales, 0);
+    quantise_kernel<T><<<grid_for(rows * blocks * 4), 256, 0, st>>>((const T*)x, pitch, rows, width, blocks, reads_wide<T>(x, pitch), codes, scales);
     CS_HIP(hipGetLastError());
     return CS_OK;
 }
@@ -210,9 +278,16 @@ int dequantise(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_
 template <class T>
 int linear(const void* x, int64_t pitch, int64_t rows, int64_t width, const uint8_t* codes, const uint8_t* scales, int64_t outputs, void* y, const LinearPlan& p,
            hipStream_t st) {
-    quantise_kernel<T, true><<<grid_for(p.rows_x * ((p.blocks + 15) / 16) * 64), 256, 0, st>>>((const T*)x, pitch, rows, width, p.blocks, reads_wide<T>(x, pitch), p.codes,
-                                                                                             p.scales_x, p.rows_x);
-    tile_scales_kernel<<<grid_for(p.rows_w * ((p.blocks + 15) / 16) * 4), 256, 0, st>>>(scales, outputs, p.blocks, p.scales_w, p.rows_w);
+    if (rows <= 16 && few_lds(rows, p.blocks) <= FEW_LDS) {
+        few_rows_kernel<T><<<dim3((unsigned)((outputs + 15) / 16)), 256, few_lds(rows, p.blocks), st>>>((const T*)x, pitch, (int)rows, width, (int)p.blocks,
+                                                                                                   reads_wide<T>(x, pitch), codes, scales, (int)outputs, (T*)y);
+        CS_HIP(hipGetLastError());
+        return CS_OK;
+    }
+    const int64_t padded = (p.blocks + 15) / 16 * 16;
+    const unsigned x_blocks = grid_for(p.rows_x * padded * 4), w_blocks = grid_for(p.rows_w * padded / 4);
+    prepare_kernel<T><<<x_blocks + w_blocks, 256, 0, st>>>((const T*)x, pitch, rows, width, p.blocks, reads_wide<T>(x, pitch), p.codes, p.scales_x, p.rows_x, scales, outputs,
+                                                           p.scales_w, p.rows_w, (int)x_blocks);
     CS_HIP(hipGetLastError());
     Problem q{};
     q.a = Operand{(const char*)codes, p.blocks * 16, outputs};

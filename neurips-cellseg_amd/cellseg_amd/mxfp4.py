@@ -98,7 +98,8 @@ def mxfp4_linear(x: torch.Tensor, weight: MXFP4Tensor) -> torch.Tensor:
     rows, outputs = rows_of(x), weight.shape[0]
     y = torch.empty(tuple(x.shape[:-1]) + (outputs,), dtype=x.dtype, device=x.device)
     with torch.cuda.device(x.device):
-        ws = torch.empty(lib.cs_mxfp4_linear_workspace_bytes(rows.shape[0], weight.width, outputs) or 1, dtype=torch.uint8, device=x.device)
+        size = lib.cs_mxfp4_linear_workspace_bytes(rows.shape[0], weight.width, outputs)
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
         check(lib.cs_mxfp4_linear(rows.data_ptr(), _pitch(rows), rows.shape[0], weight.width, TYPES[x.dtype], weight.codes.data_ptr(), weight.scales.data_ptr(), outputs,
-                                  y.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_ptr()), "cs_mxfp4_linear")
+                                  y.data_ptr(), ws.data_ptr() if size else None, size, _lib.stream_ptr()), "cs_mxfp4_linear")
     return y

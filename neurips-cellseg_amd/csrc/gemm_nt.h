@@ -319,19 +319,24 @@ struct Wide {
         // ---- e2m1: the scale words of a pair of slabs, 16 bytes a row, fetched one pair ahead into LDS behind the slabs; 16 words a lane go to
         // registers before the pair begins
         int scale[16], scale_tile = blockIdx.x, scale_pair = 0, scale_slot = 0;
+        const int64_t scale_pitch = (wave < 2 ? p.rows_a : p.rows_b) * 16;      // bytes of a pair
+        auto scales_of = [&](int id) {
+            const Tile t = tile_of(id, p);
+            return (const char*)(wave < 2 ? p.scales_a + (int64_t)t.m * 1024 : p.scales_b + (int64_t)t.n * 1024) + (wave & 1) * 2048;
+        };
+        const char* scale_at = KIND == E2M1 ? scales_of(scale_tile) : nullptr;
         auto load_scales = [&]() {
-            const Tile t = tile_of(scale_tile, p);
-            const int64_t row = (wave < 2 ? scale_pair * p.rows_a + (int64_t)t.m * 256 : scale_pair * p.rows_b + (int64_t)t.n * 256) + (wave & 1) * 128;
-            const char* from = (const char*)(wave < 2 ? p.scales_a : p.scales_b) + row * 16 + lane * 16;
             const unsigned dst = lds_address(lds) + (unsigned)(2 * STAGE_BYTES + scale_slot * 8192 + wave * 2048);
-            dma16(dst, from);
-            dma16(dst + 1024, from + 1024);
-            if (++scale_pair == pairs && scale_tile + stride < tiles) {
+            dma16(dst, scale_at + lane * 16);
+            dma16(dst + 1024, scale_at + lane * 16 + 1024);
+            scale_slot ^= 1;
+            if (++scale_pair < pairs) {
+                scale_at += scale_pitch;
+            } else if (scale_tile + stride < tiles) {
                 scale_pair = 0;
                 scale_tile += stride;
-            }
-            scale_pair = min(scale_pair, pairs - 1);
-            scale_slot ^= 1;
+                scale_at = scales_of(scale_tile);
+            }                                                            // behind the last tile the last pair comes again, unread
         };
         auto read_scales = [&]() {                                       // of the pair that was fetched last
             const char* from = lds + 2 * STAGE_BYTES + (scale_slot ^ 1) * 8192 + (lane & 15) * 16 + (lane >> 4) * 4;

@@ -43,13 +43,13 @@ __device__ __forceinline__ unsigned encode8(const float (&v)[8], unsigned* scale
     const int s = field > 2 ? field - 2 : 0;
     *scale = (unsigned)s;
     const float by = __builtin_bit_cast(float, (unsigned)(254 - s) << 23);   // 2^(127 - s): s <= 252, a normal number
+    // v_cvt_scalef32_pk_fp4_f32 with scale 1: two values to the nearest code, ties to even, above 6 to 6 (a comparison per border costs 14
+    // instructions a value and as much time as the memory)
     unsigned out = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float a = fabsf(v[i] * by);
-        const unsigned code = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.f);
-        out |= (code | (__builtin_bit_cast(unsigned, v[i]) >> 31 << 3)) << (4 * i);
-    }
+    out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, v[0] * by, v[1] * by, 1.f, 0);
+    out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, v[2] * by, v[3] * by, 1.f, 1);
+    out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, v[4] * by, v[5] * by, 1.f, 2);
+    out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, v[6] * by, v[7] * by, 1.f, 3);
     return out;
 }
 
@@ -58,75 +58,85 @@ __device__ __forceinline__ int64_t tile_place(int64_t row, int64_t block, int64_
     return (((block >> 4) * rows + row) * 4 + (block & 3)) * 4 + ((block >> 2) & 3);
 }
 
-// one block of 32 by 4 lanes: item i of rows x blocks x 4
+// Rows over thread blocks: one row or, where a row has fewer than 256 / 4 blocks of 32, several.  -> the thread's row and item (4 a block of 32)
+struct Place { int64_t row; int item; };
+__device__ __forceinline__ Place place_of(int64_t block, int items) {
+    if (items >= 256) return {block, (int)threadIdx.x};
+    const int rows = 256 / items, r = (int)threadIdx.x / items;
+    return {r < rows ? block * rows + r : (int64_t)1 << 62, (int)threadIdx.x - r * items};
+}
+unsigned row_blocks(int64_t rows, int64_t items) {
+    const int64_t per = items >= 256 ? 1 : 256 / items;
+    return (unsigned)((rows + per - 1) / per);
+}
+
 template <class T>
-__global__ __launch_bounds__(256) void quantise_kernel(const T* x, int64_t pitch, int64_t rows, int64_t width, int64_t blocks, bool wide, uint8_t* codes, uint8_t* scales) {
-    const int64_t total = rows * blocks * 4;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t b = i >> 2, row = b / blocks, block = b - row * blocks;
+__global__ __launch_bounds__(256) void quantise_kernel(const T* x, int64_t pitch, int64_t rows, int64_t width, int blocks, bool wide, uint8_t* codes, uint8_t* scales) {
+    const Place p = place_of(blockIdx.x, blocks * 4);
+    if (p.row >= rows) return;                                           // a block's 4 lanes go together
+    for (int i = p.item; i < blocks * 4; i += 256) {
         float v[8];
-        load8(x + row * pitch, block * 32 + (i & 3) * 8, width, wide, v);
+        load8(x + p.row * pitch, (int64_t)i * 8, width, wide, v);
         unsigned scale;
-        *(unsigned*)(codes + i * 4) = encode8(v, &scale);
-        if ((i & 3) == 0) scales[b] = (uint8_t)scale;
+        *(unsigned*)(codes + (p.row * blocks * 4 + i) * 4) = encode8(v, &scale);
+        if ((i & 3) == 0) scales[p.row * blocks + (i >> 2)] = (uint8_t)scale;
     }
 }
 
 // What the product reads: x quantised, and both operands' scales in its order (gemm_nt.h) over rows_x / rows_w rows, blocks up to a multiple of
-// 16, with scale 1 where there is no row or block.  The first `x_blocks` thread blocks take x, the others the weight's scales.
+// 16, with scale 1 where there is no row or block.  The first `x_blocks` thread blocks take x, the others 64 rows of a pair of the weight's scales.
 template <class T>
-__global__ __launch_bounds__(256) void prepare_kernel(const T* x, int64_t pitch, int64_t rows, int64_t width, int64_t blocks, bool wide, uint8_t* codes, uint8_t* scales_x,
-                                                      int64_t rows_x, const uint8_t* scales, int64_t outputs, uint8_t* scales_w, int64_t rows_w, int x_blocks) {
-    const int64_t padded = (blocks + 15) / 16 * 16;
-    if ((int)blockIdx.x < x_blocks) {
-        const int64_t total = rows_x * padded * 4;
-        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)x_blocks * 256) {
-            const int64_t b = i >> 2, row = b / padded, block = b - row * padded;
-            const int part = (int)(i & 3);
-            const bool in = row < rows && block < blocks;                // the same in a block's 4 lanes
+__global__ __launch_bounds__(256) void prepare_kernel(const T* x, int64_t pitch, int64_t rows, int64_t width, int blocks, bool wide, uint8_t* codes, uint8_t* scales_x,
+                                                      int64_t rows_x, const uint8_t* scales, int64_t outputs, uint8_t* scales_w, int64_t rows_w, unsigned x_blocks) {
+    const int padded = (blocks + 15) / 16 * 16;
+    if (blockIdx.x < x_blocks) {
+        const Place p = place_of(blockIdx.x, padded * 4);
+        if (p.row >= rows_x) return;
+        for (int i = p.item; i < padded * 4; i += 256) {
+            const bool in = p.row < rows && (i >> 2) < blocks;           // the same in a block's 4 lanes
             float v[8];
-            if (in) load8(x + row * pitch, block * 32 + part * 8, width, wide, v);
+            if (in) load8(x + p.row * pitch, (int64_t)i * 8, width, wide, v);
             else
 #pragma unroll
                 for (int k = 0; k < 8; ++k) v[k] = 0.f;
             unsigned scale;
             const unsigned code = encode8(v, &scale);
-            if (in) *(unsigned*)(codes + (row * blocks + block) * 16 + part * 4) = code;
-            if (part == 0) scales_x[tile_place(row, block, rows_x)] = (uint8_t)(in ? scale : 127u);
+            if (in) *(unsigned*)(codes + (p.row * blocks * 4 + i) * 4) = code;
+            if ((i & 3) == 0) scales_x[tile_place(p.row, i >> 2, rows_x)] = (uint8_t)(in ? scale : 127u);
         }
         return;
     }
-    const int64_t total = rows_w * (padded / 16) * 4;                    // words of 4 blocks: 4 h + g, h = 0..3
-    for (int64_t i = (int64_t)(blockIdx.x - x_blocks) * 256 + threadIdx.x; i < total; i += (int64_t)(gridDim.x - x_blocks) * 256) {
-        const int64_t g = i & 3, row = (i >> 2) % rows_w, pair = (i >> 2) / rows_w;
-        unsigned word = 0;
+    const unsigned at = blockIdx.x - x_blocks, groups = (unsigned)(rows_w / 64), pair = at / groups;
+    const int64_t row = (int64_t)(at - pair * groups) * 64 + (threadIdx.x >> 2);
+    const int g = threadIdx.x & 3;
+    unsigned word = 0;
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            const int64_t block = pair * 16 + h * 4 + g;
-            word |= (row < outputs && block < blocks ? (unsigned)scales[row * blocks + block] : 127u) << (8 * h);
-        }
-        ((unsigned*)scales_w)[i] = word;
+    for (int h = 0; h < 4; ++h) {
+        const int block = (int)pair * 16 + h * 4 + g;
+        word |= (row < outputs && block < blocks ? (unsigned)scales[row * blocks + block] : 127u) << (8 * h);
     }
+    ((unsigned*)scales_w)[(pair * rows_w + row) * 4 + g] = word;
 }
 
 template <class T>
-__global__ __launch_bounds__(256) void dequantise_kernel(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t width, int64_t blocks, bool wide, T* out) {
-    const int64_t total = rows * blocks * 4;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t b = i >> 2, row = b / blocks, c = (b - row * blocks) * 32 + (i & 3) * 8;
-        const unsigned code = *(const unsigned*)(codes + i * 4), s = scales[b];
-        const float by = s == 255u ? __builtin_nanf("") : ldexpf(1.f, (int)s - 127);
+__global__ __launch_bounds__(256) void dequantise_kernel(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t width, int blocks, bool wide, T* out) {
+    const Place p = place_of(blockIdx.x, blocks * 4);
+    if (p.row >= rows) return;
+    for (int i = p.item; i < blocks * 4; i += 256) {
+        const unsigned code = *(const unsigned*)(codes + (p.row * blocks * 4 + i) * 4), s = scales[p.row * blocks + (i >> 2)];
+        const float by = s == 255u ? __builtin_nanf("") : s == 0u ? __builtin_bit_cast(float, 1u << 22) : __builtin_bit_cast(float, s << 23);     // 2^(s - 127)
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        const f32x2 v[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, 1.f, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, 1.f, 1),
+                            __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, 1.f, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, 1.f, 3)};
         struct alignas(16) Eight { T v[8]; } e;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const unsigned q = code >> (4 * k), m = q & 7u;
-            // e2m1: exponent m / 2, mantissa m & 1; 0 and 1 (0.5) have no implicit one
-            const float a = m < 2u ? 0.5f * (float)m : __builtin_bit_cast(float, (((m >> 1) + 126u) << 23) | ((m & 1u) << 22));
-            e.v[k] = (T)((q & 8u ? -a : a) * by);
-        }
-        T* to = out + row * width + c;
-        if (wide && c + 8 <= width) *(Eight*)to = e;
-        else
+        for (int k = 0; k < 8; ++k) e.v[k] = (T)(v[k >> 1][k & 1] * by);
+        const int64_t c = (int64_t)i * 8;
+        T* to = out + p.row * width + c;
+        if (wide && c + 8 <= width) {
+            if constexpr (sizeof(T) == 2) __builtin_nontemporal_store(__builtin_bit_cast(i32x4, e), (i32x4*)to);
+            else *(Eight*)to = e;
+        } else
 #pragma unroll
             for (int k = 0; k < 8; ++k)
                 if (c + k < width) to[k] = e.v[k];
@@ -161,6 +171,8 @@ constexpr int FEW_LDS = 40 << 10;                 // 4 blocks a CU
 __host__ __device__ inline int few_pitch(int blocks) { return (blocks + 3) / 4 * 64 + 16; }      // bytes of a row's codes, off the powers of two
 int few_lds(int64_t rows, int64_t blocks) { return blocks > 4096 ? FEW_LDS + 1 : (int)(rows * (few_pitch((int)blocks) + (blocks + 3) / 4 * 4)); }
 
+bool few_rows(int64_t rows, int64_t blocks) { return rows <= 16 && few_lds(rows, blocks) <= FEW_LDS; }
+
 template <class T>
 __global__ __launch_bounds__(256) void few_rows_kernel(const T* x, int64_t pitch, int rows, int64_t width, int blocks, bool wide, const uint8_t* codes, const uint8_t* scales,
                                                        int outputs, T* y) {
@@ -168,8 +180,25 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const T* x, int64_t pitch
     __shared__ f32x4 join[4][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, steps = (blocks + 3) >> 2, cp = few_pitch(blocks), sp = steps * 4;
     char* const xs = few + rows * cp;                                    // scales of x [rows][sp]
+    // 4 runs of weights go out before x is quantised, and always 4 runs ahead of the products
+    const int g = lane >> 4, m0 = blockIdx.x * 16, m = min(m0 + (lane & 15), outputs - 1), n = (lane & 15) < rows ? lane & 15 : 0;
+    const uint8_t* wc = codes + (int64_t)m * blocks * 16;
+    const uint8_t* ws = scales + (int64_t)m * blocks;
+    i32x4 a[8];
+    int sa[8];
+    auto fetch = [&](int unit, int to) {                                 // run `unit`: steps 2 unit and 2 unit + 1 of 4 blocks; zeros behind the last
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int block = (2 * unit + h) * 4 + g, in = min(block, blocks - 1);
+            a[to * 2 + h] = *(const i32x4*)(wc + (int64_t)in * 16);
+            sa[to * 2 + h] = ws[in];
+            if (block >= blocks) a[to * 2 + h] = i32x4{0, 0, 0, 0}, sa[to * 2 + h] = 127;
+        }
+    };
+#pragma unroll
+    for (int c = 0; c < 4; ++c) fetch(wave + 4 * c, c);
     for (int i = tid; i < rows * sp * 4; i += 256) {
-        const int b = i >> 2, row = b / sp, block = b - row * sp;
+        const int row = rows == 1 ? 0 : i / (sp * 4), block = (i >> 2) - row * sp;
         float v[8];
         load8(x + row * pitch, (int64_t)block * 32 + (i & 3) * 8, width, wide, v);   // zeros behind the width
         unsigned scale;
@@ -177,25 +206,23 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const T* x, int64_t pitch
         if ((i & 3) == 0) xs[row * sp + block] = (char)scale;
     }
     __syncthreads();
-    const int g = lane >> 4, m0 = blockIdx.x * 16, m = min(m0 + (lane & 15), outputs - 1), n = (lane & 15) < rows ? lane & 15 : 0;
-    const uint8_t* wc = codes + (int64_t)m * blocks * 16;
-    const uint8_t* ws = scales + (int64_t)m * blocks;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int u = wave; 2 * u < steps; u += 4)
+    for (int u = wave; 2 * u < steps; u += 16)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int step = 2 * u + h, block = step * 4 + g;
-            const bool in = block < blocks;
-            i32x4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
-            int sa = 127, sb = 127;
-            if (in) {
-                a = *(const i32x4*)(wc + (int64_t)block * 16);
-                sa = ws[block];
-                b = *(const i32x4*)(few + n * cp + block * 16);
-                sb = (uint8_t)xs[n * sp + block];
+        for (int c = 0; c < 4; ++c) {
+            const int unit = u + 4 * c;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int block = (2 * unit + h) * 4 + g;
+                i32x4 b = {0, 0, 0, 0};
+                int sb = 127;
+                if (block < blocks) {
+                    b = *(const i32x4*)(few + n * cp + block * 16);
+                    sb = (uint8_t)xs[n * sp + block];
+                }
+                acc = mma<E2M1, 0>(a[c * 2 + h], b, acc, sa[c * 2 + h], sb);
             }
-            acc = mma<E2M1, 0>(a, b, acc, sa, sb);
+            if (2 * (unit + 16) < steps) fetch(unit + 16, c);
         }
     join[wave][lane] = acc;
     __syncthreads();
@@ -220,11 +247,6 @@ int launch_linear(hipStream_t st, Problem p, LinearEpi<T> epi) {
     return CS_OK;
 }
 
-unsigned grid_for(int64_t items) {
-    const int64_t blocks = (items + 255) / 256;
-    return (unsigned)(blocks < 8192 ? blocks : 8192);
-}
-
 struct LinearPlan {
     size_t bytes;
     uint8_t *codes, *scales_x, *scales_w;
@@ -236,6 +258,7 @@ LinearPlan make_plan(int64_t rows, int64_t width, int64_t outputs, void* base) {
     p.rows_x = (rows + 255) / 256 * 256;
     p.rows_w = (outputs + 255) / 256 * 256;
     const int64_t tiled = (p.blocks + 15) / 16 * 16;
+    if (few_rows(rows, p.blocks)) return p;
     size_t at = 0;
     auto take = [&](int64_t n) {
         uint8_t* q = base ? (uint8_t*)base + at : nullptr;
@@ -264,30 +287,31 @@ bool reads_wide(const void* x, int64_t pitch) {
 template <class T>
 int quantise(const void* x, int64_t pitch, int64_t rows, int64_t width, uint8_t* codes, uint8_t* scales, hipStream_t st) {
     const int64_t blocks = (width + 31) / 32;
-    quantise_kernel<T><<<grid_for(rows * blocks * 4), 256, 0, st>>>((const T*)x, pitch, rows, width, blocks, reads_wide<T>(x, pitch), codes, scales);
+    quantise_kernel<T><<<row_blocks(rows, blocks * 4), 256, 0, st>>>((const T*)x, pitch, rows, width, (int)blocks, reads_wide<T>(x, pitch), codes, scales);
     CS_HIP(hipGetLastError());
     return CS_OK;
 }
 template <class T>
 int dequantise(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t width, void* out, hipStream_t st) {
     const int64_t blocks = (width + 31) / 32;
-    dequantise_kernel<T><<<grid_for(rows * blocks * 4), 256, 0, st>>>(codes, scales, rows, width, blocks, reads_wide<T>(out, width), (T*)out);
+    dequantise_kernel<T><<<row_blocks(rows, blocks * 4), 256, 0, st>>>(codes, scales, rows, width, (int)blocks, reads_wide<T>(out, width), (T*)out);
     CS_HIP(hipGetLastError());
     return CS_OK;
 }
 template <class T>
 int linear(const void* x, int64_t pitch, int64_t rows, int64_t width, const uint8_t* codes, const uint8_t* scales, int64_t outputs, void* y, const LinearPlan& p,
            hipStream_t st) {
-    if (rows <= 16 && few_lds(rows, p.blocks) <= FEW_LDS) {
+    if (few_rows(rows, p.blocks)) {
         few_rows_kernel<T><<<dim3((unsigned)((outputs + 15) / 16)), 256, few_lds(rows, p.blocks), st>>>((const T*)x, pitch, (int)rows, width, (int)p.blocks,
                                                                                                    reads_wide<T>(x, pitch), codes, scales, (int)outputs, (T*)y);
         CS_HIP(hipGetLastError());
         return CS_OK;
     }
     const int64_t padded = (p.blocks + 15) / 16 * 16;
-    const unsigned x_blocks = grid_for(p.rows_x * padded * 4), w_blocks = grid_for(p.rows_w * padded / 4);
-    prepare_kernel<T><<<x_blocks + w_blocks, 256, 0, st>>>((const T*)x, pitch, rows, width, p.blocks, reads_wide<T>(x, pitch), p.codes, p.scales_x, p.rows_x, scales, outputs,
-                                                           p.scales_w, p.rows_w, (int)x_blocks);
+    const int64_t x_blocks = row_blocks(p.rows_x, padded * 4), w_blocks = p.rows_w / 64 * (padded / 16);
+    CS_REQUIRE(x_blocks + w_blocks < (int64_t)1 << 31, "mxfp4 linear: too many outputs");
+    prepare_kernel<T><<<dim3((unsigned)(x_blocks + w_blocks)), 256, 0, st>>>((const T*)x, pitch, rows, width, (int)p.blocks, reads_wide<T>(x, pitch), p.codes, p.scales_x,
+                                                                             p.rows_x, scales, outputs, p.scales_w, p.rows_w, (unsigned)x_blocks);
     CS_HIP(hipGetLastError());
     Problem q{};
     q.a = Operand{(const char*)codes, p.blocks * 16, outputs};
@@ -345,7 +369,7 @@ int cs_mxfp4_linear(const void* x, int64_t pitch, int64_t rows, int64_t width, i
     if (int rc = check_sizes(rows, width, type, "mxfp4 linear")) return rc;
     if (int rc = check_sizes(outputs, width, type, "mxfp4 linear")) return rc;
     if (!rows || !outputs) return CS_OK;
-    CS_REQUIRE(x && y && codes && scales && workspace, "mxfp4 linear: NULL pointer");
+    CS_REQUIRE(x && y && codes && scales && (workspace || !cs_mxfp4_linear_workspace_bytes(rows, width, outputs)), "mxfp4 linear: NULL pointer");
     CS_REQUIRE(((uintptr_t)codes & 15) == 0 && ((uintptr_t)y & 15) == 0, "mxfp4 linear: codes and output start at a multiple of 16 bytes");
     const LinearPlan p = make_plan(rows, width, outputs, workspace);
     if (workspace_bytes < p.bytes) {

@@ -88,9 +88,10 @@ def test_the_c_entry_refuses_small_workspaces_and_null():
     assert _lib.lib.cs_mxfp4_quantize(4096, 8, 4, 8, 5, 4096, 4096, None) == -1
     assert _lib.lib.cs_mxfp4_quantize(None, 8, 4, 8, 0, 4096, 4096, None) == -1
     assert _lib.lib.cs_mxfp4_dequantize(4098, 4096, 4, 8, 0, 4096, None) == -1
-    size = _lib.lib.cs_mxfp4_linear_workspace_bytes(4, 8, 6)
-    assert size > 0 and _lib.lib.cs_mxfp4_linear(4096, 8, 4, 8, 0, 4096, 4096, 6, 4096, 4096, size - 1, None) == -3
-    assert _lib.lib.cs_mxfp4_linear(4096, 8, 4, 8, 0, 4100, 4096, 6, 4096, 4096, size, None) == -1
+    size = _lib.lib.cs_mxfp4_linear_workspace_bytes(40, 8, 6)
+    assert size > 0 and _lib.lib.cs_mxfp4_linear(4096, 8, 40, 8, 0, 4096, 4096, 6, 4096, 4096, size - 1, None) == -3
+    assert _lib.lib.cs_mxfp4_linear(4096, 8, 40, 8, 0, 4096, 4096, 6, 4096, None, size, None) == -1
+    assert _lib.lib.cs_mxfp4_linear(4096, 8, 40, 8, 0, 4100, 4096, 6, 4096, 4096, size, None) == -1
 
 
 def test_workspaces_of_no_rows():

@@ -414,6 +414,7 @@ struct Wide {
             for (int i = 0; i < MF; ++i)
 #pragma unroll
                 for (int j = 0; j < NF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            const auto ahead = epi.template ahead<Wide>(t, tid);
             int left = last_of(t) - first_of(t) + 1;
             do {
                 step(zero);
@@ -421,7 +422,7 @@ struct Wide {
                 left -= KIND == E2M1 ? 2 : 1;
                 if (left == 0) asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");    // the last sums leave the pipe before anything reads them
             } while (left);
-            epi.template operator()<Wide>(p, t, lds + LDS_BYTES, acc);
+            epi.template operator()<Wide>(p, t, lds + LDS_BYTES, acc, ahead);
         }
         wait_loads<0>();
     }
@@ -504,6 +505,9 @@ __device__ __forceinline__ void store_tile(Tile t, char* lds, f32x4 (&acc)[R::MF
         }
 }
 
+// What an epilogue loads before its tile's products, which hide it: EPI::ahead.  This one: nothing.
+struct NoAhead {};
+
 // A kernel's body: the LDS that it needs, and its tile (Ring) or tiles (Wide)
 template <class R> struct Persistent { static constexpr bool value = false; };
 template <int KIND, bool TAIL> struct Persistent<Wide<KIND, TAIL>> { static constexpr bool value = true; };
@@ -518,8 +522,9 @@ __device__ __forceinline__ void product(const Problem& p, char* lds, const EPI& 
     } else {
         const Tile t = tile_of(blockIdx.x, p);
         f32x4 acc[R::MF][R::NF];
+        const auto ahead = epi.template ahead<R>(t, threadIdx.x);
         R::run(p, t, lds, acc);
-        epi.template operator()<R>(p, t, lds, acc);
+        epi.template operator()<R>(p, t, lds, acc, ahead);
     }
 }
 

@@ -26,105 +26,136 @@ template <> struct Elem<FP32> { typedef float T; static constexpr float G_SCALE 
 
 // what the forward pass leaves for the backward pass
 struct Saved {
-    float2* norm;      // [rows] maximum of z, 1 / sum exp((z - maximum) / T)
+    float2* norm;      // [rows] M, 1 / sum_j 2^(c z_j - M);  c = log2(e) / T, M = the largest c z_j rounded up
     int* state;        // [rows] RowState
     float* inv_count;  // [1]
-    int* ids;          // [rows][top] ascending, each id once, NO_ID behind the last
+    int* ids;          // [rows][top] ascending, each id once, NO_ID behind the last (a target that does not count: NO_ID)
     float* q;          // [rows][top] (distillation)
     float* z;          // [rows][top]
     uint16_t* starts;  // [rows][starts_pitch] distillation: how many ids of the row lie below 128 t
     int64_t starts_pitch;
 };
 
-// Where a row's ascending list of ids has those of a tile's m0 .. m0 + size: positions lo .. hi.  The cross entropy has one id a row; a
-// list has its positions at the multiples of 128 beside it, so that no tile searches.
-template <bool LIST>
-__device__ __forceinline__ int2 listed_range(const Saved& s, int64_t n, int from, int size) {
-    if constexpr (LIST) {
-        const uint16_t* at = s.starts + n * s.starts_pitch + (from >> 7);
-        return make_int2(at[0], at[size >> 7]);
-    } else {
-        return make_int2(0, (unsigned)(s.ids[n] - from) < (unsigned)size ? 1 : 0);
-    }
+__device__ __forceinline__ int64_t id_at(const void* ids, int bits, int64_t i) {
+    return bits == 64 ? ((const int64_t*)ids)[i] : (int64_t)((const int*)ids)[i];
+}
+struct Targets {       // of the cross entropy, as the caller has them
+    const void* ids;
+    int bits;
+    int64_t pitch, ignore;
+};
+
+// The listed ids of a row that fall into a tile's from .. from + size: positions x .. y of its ascending list, from the table beside the list, so
+// that no tile searches.  One thread per row looks them up before the tile's products and puts them, with what belongs to the first, into LDS:
+// a wave that met them one fragment after the other would wait for each (a row of 64 ids has one in a tile of 50 000 / 256 every third time,
+// seldom a second).
+__device__ __forceinline__ int2 listed_of(const Saved& s, int64_t n, int from, int size) {
+    const uint16_t* at = s.starts + n * s.starts_pitch + (from >> 7);
+    return make_int2(at[0], at[size >> 7]);
 }
 
-// ---- forward: maximum and sum of exponentials of a tile's rows, and the listed z ---------------------------------------------------
+// ---- forward: of a tile's rows M, the largest c z rounded up, and the sum of 2^(c z - M); and the listed z ----------------------------
+// M is a whole number: c z - M is one rounding from exact, and sums of different M join by exact powers of two.
 template <bool LIST>
 struct NormEpi {
     float2* part;      // [rows][tiles_m]
     Saved s;
+    Targets targets;   // cross entropy
     int rows, vocab, top;
     float c;           // log2(e) / T
-    template <class R> static constexpr int lds() { return R::WAVES_M * R::TILE_N * 8; }
+    struct Row { int lo, hi, first, none; };
+    template <class R> static constexpr int lds() { return R::TILE_N * (int)sizeof(Row) + R::WAVES_M * R::TILE_N * 8; }
     template <class R>
-    __device__ __forceinline__ void operator()(const Problem& p, Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF]) const {
+    __device__ __forceinline__ Row ahead(Tile t, int tid) const {
+        Row r{};
+        if (tid < R::TILE_N) {
+            const int n = t.n * R::TILE_N + tid, in = min(n, rows - 1), m0 = t.m * R::TILE_M;
+            if constexpr (LIST) {
+                const int2 at = listed_of(s, in, m0, R::TILE_M);
+                r = {at.x, n < rows ? at.y : at.x, 0, 0};
+            } else {
+                const int64_t id = id_at(targets.ids, targets.bits, in * targets.pitch);
+                r = {0, n < rows && id >= m0 && id < m0 + R::TILE_M ? 1 : 0, (int)id, 0};
+            }
+        }
+        return r;
+    }
+    template <class R>
+    __device__ __forceinline__ void operator()(const Problem& p, Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF], Row mine) const {
+        static_assert(R::TILE_N <= R::THREADS, "");
         const int tid = fresh(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / R::WAVES_N, wn = wave % R::WAVES_N;
         const int m0 = t.m * R::TILE_M, n0 = t.n * R::TILE_N;
-        float2* join = (float2*)lds;                                     // [WAVES_M][TILE_N]
+        Row* info = (Row*)lds;                                           // [TILE_N]
+        float2* join = (float2*)(lds + R::TILE_N * sizeof(Row));         // [WAVES_M][TILE_N]
         const int g4 = (lane >> 4) * 4;
         hold<R>(acc, 0);
-        int2 range[R::NF];
-#pragma unroll
-        for (int j = 0; j < R::NF; ++j) {
-            const int n = n0 + R::col0(wn, j) + (lane & 15);
-            range[j] = listed_range<LIST>(s, min(n, rows - 1), m0, R::TILE_M);      // no branch around the loads: they go out together
-            if (n >= rows) range[j].y = range[j].x;
+        if (tid < R::TILE_N) {
+            if (LIST && mine.lo < mine.hi) mine.first = s.ids[(int64_t)(n0 + tid) * top + mine.lo];
+            info[tid] = mine;
         }
+        if (m0 + R::TILE_M > vocab) {                                    // behind the last word
+#pragma unroll
+            for (int j = 0; j < R::NF; ++j)
+#pragma unroll
+                for (int i = 0; i < R::MF; ++i) {
+                    f32x4 v = take(acc[i][j]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) v[r] = m0 + R::row0(wm, i) + g4 + r < vocab ? v[r] : -INFINITY;
+                    give(acc[i][j], v);
+                }
+        }
+        lds_barrier();
 #pragma unroll
         for (int j = 0; j < R::NF; ++j) {
             f32x4 v[R::MF];
             hold<R>(acc, j);
 #pragma unroll
-            for (int i = 0; i < R::MF; ++i) {
-                v[i] = take(acc[i][j]);
-                if (m0 + R::TILE_M > vocab)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) v[i][r] = m0 + R::row0(wm, i) + g4 + r < vocab ? v[i][r] : -INFINITY;
-            }
-            float m = -INFINITY, sum = 0.f;
+            for (int i = 0; i < R::MF; ++i) v[i] = take(acc[i][j]);
+            float m = -INFINITY, sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < R::MF; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) m = fmaxf(m, v[i][r]);
             m = fmaxf(m, __shfl_xor(m, 16));
-            m = fmaxf(m, __shfl_xor(m, 32));
+            m = ceilf(fmaxf(m, __shfl_xor(m, 32)) * c);
             const float at = m == -INFINITY ? 0.f : m;                   // no value above -inf: the sum is 0, not NaN
 #pragma unroll
             for (int i = 0; i < R::MF; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f((v[i][r] - at) * c);
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            if (lane < 16) join[wm * R::TILE_N + R::col0(wn, j) + lane] = make_float2(m, sum);
+                for (int r = 0; r < 4; ++r) sum[r] += __builtin_amdgcn_exp2f(fmaf(v[i][r], c, -at));
+            sum[0] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            sum[0] += __shfl_xor(sum[0], 16);
+            sum[0] += __shfl_xor(sum[0], 32);
+            if (lane < 16) join[wm * R::TILE_N + R::col0(wn, j) + lane] = make_float2(m, sum[0]);
+            const Row listed = info[R::col0(wn, j) + (lane & 15)];
             const int64_t row = (int64_t)(n0 + R::col0(wn, j) + (lane & 15)) * top;
-            for (int e = range[j].x; e < range[j].y; ++e) {
-                const int want = s.ids[row + e] - m0 - g4;
+            for (int e = listed.lo; e < listed.hi; ++e) {
+                const int want = (e == listed.lo ? listed.first : s.ids[row + e]) - m0 - g4;
                 float z = 0.f;
-                bool mine = false;
+                bool here = false;
 #pragma unroll
                 for (int i = 0; i < R::MF; ++i)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         if (want == R::row0(wm, i) + r) {
                             z = v[i][r];
-                            mine = true;
+                            here = true;
                         }
-                if (mine) s.z[row + e] = z;
+                if (here) s.z[row + e] = z;
             }
         }
         lds_barrier();
-        for (int i = tid; i < R::TILE_N; i += R::THREADS) {
-            if (n0 + i >= rows) continue;
+        if (tid < R::TILE_N && n0 + tid < rows) {
             float m = -INFINITY, sum = 0.f;
 #pragma unroll
-            for (int w = 0; w < R::WAVES_M; ++w) m = fmaxf(m, join[w * R::TILE_N + i].x);
+            for (int w = 0; w < R::WAVES_M; ++w) m = fmaxf(m, join[w * R::TILE_N + tid].x);
             const float at = m == -INFINITY ? 0.f : m;
 #pragma unroll
             for (int w = 0; w < R::WAVES_M; ++w) {
-                const float2 v = join[w * R::TILE_N + i];
-                sum += v.x == -INFINITY ? v.y : v.y * __builtin_amdgcn_exp2f((v.x - at) * c);
+                const float2 v = join[w * R::TILE_N + tid];
+                sum += v.x == -INFINITY ? v.y : v.y * __builtin_amdgcn_exp2f(v.x - at);
             }
-            part[(int64_t)(n0 + i) * p.tiles_m + t.m] = make_float2(m, sum);
+            part[(int64_t)(n0 + tid) * p.tiles_m + t.m] = make_float2(m, sum);
         }
     }
 };
@@ -132,6 +163,23 @@ struct NormEpi {
 // ---- backward: G = p - q of a piece of the vocabulary, and its transpose ----------------------------------------------------------
 // The listed entries come from the z of the forward pass, p - q in fp32 before the one rounding.  Both matrices leave through LDS, 16 rows (fp32: 8)
 // of a wave's tile at a time, as whole lines and past the caches: see store_tile.
+template <class T> struct alignas(4 * sizeof(T)) Four { T v[4]; };
+// 4 values rounded to T, or zeros whatever they are where `keep` is 0
+template <class T>
+__device__ __forceinline__ Four<T> pack(f32x4 v, unsigned keep) {
+    if constexpr (sizeof(T) == 2) {
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        typedef T Tx2 __attribute__((ext_vector_type(2)));
+        const uint2 w = make_uint2(__builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){v[0], v[1]}, Tx2)) & keep,
+                                   __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){v[2], v[3]}, Tx2)) & keep);
+        return __builtin_bit_cast(Four<T>, w);
+    } else {
+        i32x4 w = __builtin_bit_cast(i32x4, v);
+        w &= i32x4{(int)keep, (int)keep, (int)keep, (int)keep};
+        return __builtin_bit_cast(Four<T>, w);
+    }
+}
+
 template <int KIND, bool LIST>
 struct GradEpi {
     typedef typename Elem<KIND>::T T;
@@ -141,11 +189,17 @@ struct GradEpi {
     Saved s;
     int rows, from, size, top;     // this piece: ids from .. from + size
     float c;
+    // fragment columns that go together: 64 rows are a line of a 16-bit G^T, and all 128 at once do not fit the registers
+    template <class R> static constexpr int group() { return R::NF < 4 ? R::NF : 4; }
     template <class R> static constexpr int wave_lds() {
-        constexpr int m = R::TILE_M / R::WAVES_M, n = R::TILE_N / R::WAVES_N;
-        return Stage<T, (m > n ? m : n)>::BYTES;
+        return Stage<T, (R::TILE_M / R::WAVES_M > 16 * group<R>() ? R::TILE_M / R::WAVES_M : 16 * group<R>())>::BYTES;
     }
-    template <class R> static constexpr int lds() { return R::WAVES_M * R::WAVES_N * wave_lds<R>(); }
+    struct alignas(16) Row { float m, inv; unsigned keep; int lo, hi, first; float d, none; };   // keep: 0 for a row that does not count, else ~0; d: G at the first listed id
+    template <class R> static constexpr int lds() { return R::TILE_N * (int)sizeof(Row) + R::WAVES_M * R::WAVES_N * wave_lds<R>(); }
+    // p - q of a listed entry
+    __device__ __forceinline__ float grad_at(float m, float inv, int64_t entry) const {
+        return (__builtin_amdgcn_exp2f(fmaf(s.z[entry], c, -m)) * inv - (LIST ? s.q[entry] : 1.f)) * Elem<KIND>::G_SCALE;
+    }
     // staged rows of N elements -> memory
     template <int N>
     __device__ __forceinline__ static void put(const char* stage, T* to, int64_t pitch, int lane) {
@@ -160,79 +214,126 @@ struct GradEpi {
         wave_sync();
     }
     template <class R>
-    __device__ __forceinline__ void operator()(const Problem& p, Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF]) const {
-        constexpr int TM = R::TILE_M / R::WAVES_M, TN = R::TILE_N / R::WAVES_N;
+    __device__ __forceinline__ Row ahead(Tile t, int tid) const {
+        Row r{};
+        if (tid < R::TILE_N) {
+            const int n = t.n * R::TILE_N + tid, in = min(n, rows - 1), m0 = t.m * R::TILE_M;
+            const float2 norm = s.norm[in];
+            const int state = n < rows ? s.state[in] : ROW_SKIP;
+            int2 at;
+            if constexpr (LIST) {
+                at = listed_of(s, in, from + m0, R::TILE_M);
+            } else {
+                r.first = s.ids[in];
+                r.d = s.z[in];                                           // z so far
+                at = make_int2(0, (unsigned)(r.first - from - m0) < (unsigned)R::TILE_M ? 1 : 0);
+            }
+            r.m = norm.x;
+            r.inv = state == ROW_BAD ? __builtin_nanf("") : norm.y;
+            r.keep = state == ROW_SKIP ? 0u : ~0u;
+            r.lo = at.x;
+            r.hi = state == ROW_COUNT ? at.y : at.x;
+        }
+        return r;
+    }
+    template <class R>
+    __device__ __forceinline__ void operator()(const Problem& p, Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF], Row mine) const {
+        constexpr int TM = R::TILE_M / R::WAVES_M, JG = group<R>(), TN = 16 * JG;
+        static_assert(R::TILE_N <= R::THREADS, "");
         const int tid = fresh(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / R::WAVES_N, wn = wave % R::WAVES_N;
         const int m0 = t.m * R::TILE_M, n0 = t.n * R::TILE_N, g4 = (lane >> 4) * 4, col = lane & 15;
-        char* stage = lds + wave * wave_lds<R>();
-        struct alignas(4 * sizeof(T)) Four { T v[4]; };
+        Row* info = (Row*)lds;                                           // [TILE_N]
+        char* stage = lds + R::TILE_N * sizeof(Row) + wave * wave_lds<R>();
         hold<R>(acc, 0);
-        int2 range[R::NF];
-        int state[R::NF];
-        float2 norm[R::NF];
-#pragma unroll
-        for (int j = 0; j < R::NF; ++j) {
-            const int n = n0 + R::col0(wn, j) + col;
-            const int at = min(n, rows - 1);                             // no branch around the loads: they go out together
-            state[j] = s.state[at];
-            norm[j] = s.norm[at];
-            range[j] = listed_range<LIST>(s, at, from + m0, R::TILE_M);
-            if (n >= rows) state[j] = ROW_SKIP;
+        if (tid < R::TILE_N) {
+            const int64_t first = (int64_t)(n0 + tid) * top + mine.lo;
+            if constexpr (LIST) {
+                if (mine.lo < mine.hi) {
+                    mine.first = s.ids[first];
+                    mine.d = grad_at(mine.m, mine.inv, first);
+                }
+            } else {
+                mine.d = (__builtin_amdgcn_exp2f(fmaf(mine.d, c, -mine.m)) * mine.inv - 1.f) * Elem<KIND>::G_SCALE;
+            }
+            mine.inv *= Elem<KIND>::G_SCALE;
+            info[tid] = mine;
         }
+        lds_barrier();
         typedef Stage<T, TM> SG;
         typedef Stage<T, TN> ST;
-        Four packed[R::MF][R::NF];                                       // 32-bit: as many registers as the sums took
 #pragma unroll
-        for (int j = 0; j < R::NF; ++j) {
-            f32x4 v[R::MF];
-            hold<R>(acc, j);
-            const float inv = state[j] == ROW_BAD ? __builtin_nanf("") : norm[j].y * Elem<KIND>::G_SCALE;
+        for (int j0 = 0; j0 < R::NF; j0 += JG) {
+            Four<T> packed[R::MF][JG];
 #pragma unroll
-            for (int i = 0; i < R::MF; ++i) {
-                v[i] = take(acc[i][j]);
+            for (int jj = 0; jj < JG; ++jj) {
+                const int j = j0 + jj;
+                f32x4 v[R::MF];
+                hold<R>(acc, j);
+                const Row info_j = info[R::col0(wn, j) + col];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float e = __builtin_amdgcn_exp2f((v[i][r] - norm[j].x) * c) * inv;
-                    v[i][r] = state[j] == ROW_SKIP || m0 + R::row0(wm, i) + g4 + r >= size ? 0.f : e;
-                }
-            }
-            const int64_t row = (int64_t)(n0 + R::col0(wn, j) + col) * top;
-            if (state[j] == ROW_COUNT)
-                for (int e = range[j].x; e < range[j].y; ++e) {
-                    const int want = s.ids[row + e] - from - m0 - g4;
-                    const float q = LIST ? s.q[row + e] : 1.f;              // the cross entropy: 1
-                    const float d = (__builtin_amdgcn_exp2f((s.z[row + e] - norm[j].x) * c) * norm[j].y - q) * Elem<KIND>::G_SCALE;
+                for (int i = 0; i < R::MF; ++i) v[i] = take(acc[i][j]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int i = 0; i < R::MF; ++i) v[i][r] = __builtin_amdgcn_exp2f(fmaf(v[i][r], c, -info_j.m));
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int i = 0; i < R::MF; ++i) v[i][r] *= info_j.inv;
+                const int64_t row = (int64_t)(n0 + R::col0(wn, j) + col) * top;
+                for (int e = info_j.lo; e < info_j.hi; ++e) {
+                    const int want = (e == info_j.lo ? info_j.first : s.ids[row + e]) - from - m0 - g4;
+                    const float d = e == info_j.lo ? info_j.d : grad_at(info_j.m, info_j.inv * (1.f / Elem<KIND>::G_SCALE), row + e);
 #pragma unroll
                     for (int i = 0; i < R::MF; ++i)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) v[i][r] = want == R::row0(wm, i) + r ? d : v[i][r];
                 }
-            T* to = g + (int64_t)(n0 + R::col0(wn, j)) * pitch_g + m0 + R::row0(wm, 0);
+                T* to = g + (int64_t)(n0 + R::col0(wn, j)) * pitch_g + m0 + R::row0(wm, 0);
 #pragma unroll
-            for (int i = 0; i < R::MF; ++i) packed[i][j] = Four{{(T)v[i][0], (T)v[i][1], (T)v[i][2], (T)v[i][3]}};
+                for (int i = 0; i < R::MF; ++i) packed[i][jj] = pack<T>(v[i], info_j.keep);
+                if (m0 + R::TILE_M > size)                               // behind the piece's last id
 #pragma unroll
-            for (int part = 0; part < 16; part += SG::ROWS) {
+                    for (int i = 0; i < R::MF; ++i)
 #pragma unroll
-                for (int i = 0; i < R::MF; ++i)
-                    if (SG::ROWS == 16 || (col & ~(SG::ROWS - 1)) == part) *(Four*)(stage + SG::at(col & (SG::ROWS - 1), (i * 16 + g4) * (int)sizeof(T))) = packed[i][j];
-                put<TM>(stage, to + part * pitch_g, pitch_g, lane);
+                        for (int r = 0; r < 4; ++r)
+                            if (m0 + R::row0(wm, i) + g4 + r >= size) packed[i][jj].v[r] = (T)0.f;
+#pragma unroll
+                for (int part = 0; part < 16; part += SG::ROWS) {
+#pragma unroll
+                    for (int i = 0; i < R::MF; ++i)
+                        if (SG::ROWS == 16 || (col & ~(SG::ROWS - 1)) == part) *(Four<T>*)(stage + SG::at(col & (SG::ROWS - 1), (i * 16 + g4) * (int)sizeof(T))) = packed[i][jj];
+                    put<TM>(stage, to + part * pitch_g, pitch_g, lane);
+                }
             }
-        }
-        if (!gt) return;
+            if (!gt) continue;
 #pragma unroll
-        for (int i = 0; i < R::MF; ++i) {
-            T* to = gt + (int64_t)(m0 + R::row0(wm, i)) * pitch_gt + n0 + R::col0(wn, 0);
+            for (int i = 0; i < R::MF; ++i) {
+                T* to = gt + (int64_t)(m0 + R::row0(wm, i)) * pitch_gt + n0 + R::col0(wn, j0);
 #pragma unroll
-            for (int part = 0; part < 16; part += ST::ROWS) {
+                for (int part = 0; part < 16; part += ST::ROWS) {
 #pragma unroll
-                for (int j = 0; j < R::NF; ++j)
+                    for (int j = 0; j < JG; ++j)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (ST::ROWS == 16 || (g4 & ~(ST::ROWS - 1)) == part) *(T*)(stage + ST::at((g4 + r) & (ST::ROWS - 1), (j * 16 + col) * (int)sizeof(T))) = packed[i][j].v[r];
-                put<TN>(stage, to + part * pitch_gt, pitch_gt, lane);
+                        for (int r = 0; r < 4; ++r)
+                            if (ST::ROWS == 16 || (g4 & ~(ST::ROWS - 1)) == part) *(T*)(stage + ST::at((g4 + r) & (ST::ROWS - 1), (j * 16 + col) * (int)sizeof(T))) = packed[i][j].v[r];
+                    put<TN>(stage, to + part * pitch_gt, pitch_gt, lane);
+                }
             }
         }
     }
+};
+
+// ---- the factor of every row.  dH of row n is hidden(n) (G W)_n; dW sums weight_row(n) h_n and is multiplied by weight().  A gradient per row is
+// divided by the largest, so that 16-bit copies of h keep their range (row_scale_kernel).  Rows that do not count get 0 by selection.
+struct Factors {
+    const float *grad, *inv_count;     // one gradient for all rows
+    const int* state;
+    const float *to_h, *in_w, *w_scale;    // one per row; else NULL
+    float f;                           // T / Elem::G_SCALE
+    __device__ __forceinline__ float hidden(int64_t n) const { return to_h ? to_h[n] : state[n] != ROW_SKIP ? *grad * *inv_count * f : 0.f; }
+    __device__ __forceinline__ float weight_row(int64_t n) const { return in_w ? in_w[n] : state[n] != ROW_SKIP ? 1.f : 0.f; }
+    __device__ __forceinline__ float weight() const { return w_scale ? *w_scale : *grad * *inv_count * f; }
 };
 
 // ---- dH: fp32 sums over the pieces ------------------------------------------------------------------------------------------------
@@ -241,8 +342,9 @@ struct SumEpi {
     int rows, width;
     bool add;
     template <class R> static constexpr int lds() { return stage_bytes<R, float>(); }
+    template <class R> __device__ __forceinline__ NoAhead ahead(Tile, int) const { return {}; }
     template <class R>
-    __device__ __forceinline__ void operator()(const Problem& p, Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF]) const {
+    __device__ __forceinline__ void operator()(const Problem& p, Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF], NoAhead) const {
         store_tile<R>(t, lds, acc, out + (int64_t)t.split * rows * width, width, rows, width, add, [](float v) { return v; });
     }
 };
@@ -253,11 +355,12 @@ struct OutEpi {
     typedef typename Elem<KIND>::T T;
     T* out;            // [rows of n][width]
     int rows, width;
-    const float* scale;
+    Factors factors;
     template <class R> static constexpr int lds() { return stage_bytes<R, T>(); }
+    template <class R> __device__ __forceinline__ NoAhead ahead(Tile, int) const { return {}; }
     template <class R>
-    __device__ __forceinline__ void operator()(const Problem& p, Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF]) const {
-        const float f = *scale;
+    __device__ __forceinline__ void operator()(const Problem& p, Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF], NoAhead) const {
+        const float f = factors.weight();
         store_tile<R>(t, lds, acc, out, width, rows, width, false, [f](float v) { return v * f; });
     }
 };
@@ -308,20 +411,6 @@ int launch_product(hipStream_t st, Shape sh, const Operand& a, const Operand& b,
 }
 
 // ---- rows ---------------------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ int64_t id_at(const void* ids, int bits, int64_t i) {
-    return bits == 64 ? ((const int64_t*)ids)[i] : (int64_t)((const int*)ids)[i];
-}
-
-__global__ __launch_bounds__(256) void target_rows_kernel(const void* ids, int bits, int64_t pitch, int64_t rows, int64_t vocab, int64_t ignore, Saved s) {
-    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (n >= rows) return;
-    const int64_t t = id_at(ids, bits, n * pitch);
-    const bool skip = t == ignore, good = !skip && t >= 0 && t < vocab;
-    s.state[n] = skip ? ROW_SKIP : good ? ROW_COUNT : ROW_BAD;
-    s.ids[n] = good ? (int)t : NO_ID;
-    s.z[n] = 0.f;
-}
-
 __device__ __forceinline__ float teacher_at(const void* p, int type, int64_t i) {
     if (type == CS_TYPE_BF16) return (float)((const __bf16*)p)[i];
     if (type == CS_TYPE_FP16) return (float)((const _Float16*)p)[i];
@@ -444,13 +533,22 @@ __global__ __launch_bounds__(256) void teacher_rows_kernel(const void* ids, int 
         }
 }
 
-// A wave per row: joins the tiles' maxima and sums, in 64 bits, into the row's loss.
-__global__ __launch_bounds__(256) void row_loss_kernel(const float2* part, int tiles, int64_t rows, int top, bool listed_q, float c, double t, const double* entropy,
-                                                       Saved s, double* losses, float* out) {
-    const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (n >= rows) return;
+// One row by one wave: joins the tiles' maxima and sums, in 64 bits, into the row's loss -> in lane 0: the loss, and what the backward pass needs
+template <bool LIST>
+__device__ __forceinline__ double row_loss(int64_t n, int lane, const float2* part, int tiles, int top, int64_t vocab, float c, double t, const double* entropy,
+                                           const Targets& targets, const Saved& s, int* counted) {
     const float2* row = part + n * tiles;
+    int state;
+    if constexpr (LIST) {
+        state = s.state[n];
+    } else {
+        const int64_t id = id_at(targets.ids, targets.bits, n * targets.pitch);
+        state = id == targets.ignore ? ROW_SKIP : id >= 0 && id < vocab ? ROW_COUNT : ROW_BAD;
+        if (lane == 0) {
+            s.state[n] = state;
+            s.ids[n] = state == ROW_COUNT ? (int)id : NO_ID;
+        }
+    }
     float m = -INFINITY;
     for (int i = lane; i < tiles; i += 64) m = fmaxf(m, row[i].x);
 #pragma unroll
@@ -459,52 +557,41 @@ __global__ __launch_bounds__(256) void row_loss_kernel(const float2* part, int t
     double sum = 0.0, named = 0.0;
     for (int i = lane; i < tiles; i += 64) {
         const float2 v = row[i];
-        sum += v.x == -INFINITY ? (double)v.y : (double)v.y * (double)__builtin_amdgcn_exp2f((v.x - at) * c);
+        sum += v.x == -INFINITY ? (double)v.y : ldexp((double)v.y, (int)fmaxf(v.x - at, -2000.f));
     }
-    for (int i = lane; i < top; i += 64)
-        if (s.ids[n * top + i] != NO_ID) {
-            const float q = listed_q ? s.q[n * top + i] : 1.f;
-            if (q > 0.f || q != q) named += (double)q * (double)s.z[n * top + i];
-        }
+    if constexpr (LIST) {
+        for (int i = lane; i < top; i += 64)
+            if (s.ids[n * top + i] != NO_ID) {
+                const float q = s.q[n * top + i];
+                if (q > 0.f || q != q) named += (double)q * (double)s.z[n * top + i];
+            }
+    } else if (lane == 0 && state == ROW_COUNT) {
+        named = (double)s.z[n];
+    }
 #pragma unroll
     for (int x = 32; x; x >>= 1) {
         sum += __shfl_xor(sum, x);
         named += __shfl_xor(named, x);
     }
-    if (lane == 0) {
-        const int state = s.state[n];
-        const double h = listed_q ? entropy[n] : 0.0;
-        double loss = t * t * (h + log(sum) + ((double)m - named) / t);
-        if (state == ROW_SKIP) loss = 0.0;
-        if (state == ROW_BAD) loss = (double)__builtin_nanf("");
-        s.norm[n] = make_float2(m, (float)(1.0 / sum));
-        losses[n] = loss;
-        if (out) out[n] = (float)loss;
-    }
+    // in units of 1 / T as the kernels have it, c ln 2
+    double loss = t * t * ((LIST ? entropy[n] : 0.0) + log(sum) + ((double)m - named * (double)c) * 0.69314718055994531);
+    if (state == ROW_SKIP) loss = 0.0;
+    if (state == ROW_BAD) loss = (double)__builtin_nanf("");
+    if (lane == 0) s.norm[n] = make_float2(m, (float)(1.0 / sum));
+    *counted = state != ROW_SKIP;
+    return loss;
 }
 
-// one block: the sum over the rows in a fixed order
-__global__ __launch_bounds__(1024) void reduce_loss_kernel(const double* losses, const int* state, int64_t rows, bool mean, float* loss, float* inv_count) {
+// the sum over a block's 16 waves, in their order
+__device__ __forceinline__ void reduce_block(double sum, int count, bool mean, float* loss, float* inv_count) {
     __shared__ double sums[16];
     __shared__ int counts[16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    double sum = 0.0;
-    int count = 0;
-    for (int64_t n = tid; n < rows; n += 1024) {
-        sum += losses[n];
-        count += state[n] != ROW_SKIP;
-    }
-#pragma unroll
-    for (int x = 32; x; x >>= 1) {
-        sum += __shfl_xor(sum, x);
-        count += __shfl_xor(count, x);
-    }
-    if (lane == 0) {
-        sums[wave] = sum;
-        counts[wave] = count;
+    if ((threadIdx.x & 63) == 0) {
+        sums[threadIdx.x >> 6] = sum;
+        counts[threadIdx.x >> 6] = count;
     }
     __syncthreads();
-    if (tid == 0) {
+    if (threadIdx.x == 0) {
         sum = 0.0;
         count = 0;
         for (int w = 0; w < 16; ++w) {
@@ -517,38 +604,79 @@ __global__ __launch_bounds__(1024) void reduce_loss_kernel(const double* losses,
     }
 }
 
-// One block: the factor of every row.  dH of row n is to_h[n] (G W)_n; dW sums in_w[n] h_n, |in_w| <= 1, and is multiplied by *w_scale: a
-// gradient per row is divided by the largest, so that fp16 copies of h keep their range.  Rows that do not count get 0 by selection.
-__global__ __launch_bounds__(1024) void row_scale_kernel(const float* grad, int64_t stride, bool per_row, const int* state, const float* inv_count, int64_t rows,
-                                                         float t, float inv_g, float* to_h, float* in_w, float* w_scale) {
+template <bool LIST>
+__global__ __launch_bounds__(256) void row_loss_kernel(const float2* part, int tiles, int64_t rows, int top, int64_t vocab, float c, double t, const double* entropy,
+                                                       Targets targets, Saved s, double* losses, float* out) {
+    const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (n >= rows) return;
+    int counted;
+    const double loss = row_loss<LIST>(n, threadIdx.x & 63, part, tiles, top, vocab, c, t, entropy, targets, s, &counted);
+    if ((threadIdx.x & 63) == 0) {
+        losses[n] = loss;
+        if (out) out[n] = (float)loss;
+    }
+}
+
+// one block: the sum over the rows in a fixed order
+__global__ __launch_bounds__(1024) void reduce_loss_kernel(const double* losses, const int* state, int64_t rows, bool mean, float* loss, float* inv_count) {
+    double sum = 0.0;
+    int count = 0;
+    for (int64_t n = threadIdx.x; n < rows; n += 1024) {
+        sum += losses[n];
+        count += state[n] != ROW_SKIP;
+    }
+#pragma unroll
+    for (int x = 32; x; x >>= 1) {
+        sum += __shfl_xor(sum, x);
+        count += __shfl_xor(count, x);
+    }
+    reduce_block(sum, count, mean, loss, inv_count);
+}
+
+// both for few rows, in one launch of one block
+constexpr int FEW_ROWS = 64;
+template <bool LIST>
+__global__ __launch_bounds__(1024) void few_losses_kernel(const float2* part, int tiles, int rows, int top, int64_t vocab, float c, double t, const double* entropy,
+                                                          Targets targets, Saved s, float* out, bool mean, float* loss, float* inv_count) {
+    double sum = 0.0;
+    int count = 0;
+    for (int n = threadIdx.x >> 6; n < rows; n += 16) {
+        int counted;
+        const double one = row_loss<LIST>(n, threadIdx.x & 63, part, tiles, top, vocab, c, t, entropy, targets, s, &counted);
+        if (out && (threadIdx.x & 63) == 0) out[n] = (float)one;
+        sum += one;
+        count += counted;
+    }
+    reduce_block(sum, count, mean, loss, inv_count);
+}
+
+// One block: the factors where every row has a gradient of its own
+__global__ __launch_bounds__(1024) void row_scale_kernel(const float* grad, int64_t stride, const int* state, int64_t rows, float f, float* to_h, float* in_w, float* w_scale) {
     __shared__ float most[16];
     const int tid = threadIdx.x;
     float big = 0.f;
-    if (per_row) {
-        for (int64_t n = tid; n < rows; n += 1024)
-            if (state[n] != ROW_SKIP) big = fmaxf(big, fabsf(grad[n * stride]));
+    for (int64_t n = tid; n < rows; n += 1024)
+        if (state[n] != ROW_SKIP) big = fmaxf(big, fabsf(grad[n * stride]));
 #pragma unroll
-        for (int x = 32; x; x >>= 1) big = fmaxf(big, __shfl_xor(big, x));
-        if ((tid & 63) == 0) most[tid >> 6] = big;
-        __syncthreads();
-        big = most[0];
-        for (int w = 1; w < 16; ++w) big = fmaxf(big, most[w]);
-    }
-    const float one = per_row ? 1.f : *grad * *inv_count, f = t * inv_g;
+    for (int x = 32; x; x >>= 1) big = fmaxf(big, __shfl_xor(big, x));
+    if ((tid & 63) == 0) most[tid >> 6] = big;
+    __syncthreads();
+    big = most[0];
+    for (int w = 1; w < 16; ++w) big = fmaxf(big, most[w]);
     for (int64_t n = tid; n < rows; n += 1024) {
         const bool live = state[n] != ROW_SKIP;
-        const float g = per_row ? grad[n * stride] : one;
+        const float g = grad[n * stride];
         to_h[n] = live ? g * f : 0.f;
-        in_w[n] = !live ? 0.f : !per_row ? 1.f : big == 0.f ? g : g / big;
+        in_w[n] = !live ? 0.f : big == 0.f ? g : g / big;
     }
-    if (tid == 0) *w_scale = (per_row ? (big == 0.f ? 1.f : big) : one) * f;
+    if (tid == 0) *w_scale = (big == 0.f ? 1.f : big) * f;
 }
 
-// src [rows][cols] (element pitch) -> dst [cols][pitch], columns of dst behind the rows zero up to `padded`; row n times scale[n] (NULL: 1; 0 selects 0).
+// src [rows][cols] (element pitch) -> dst [cols][pitch], columns of dst behind the rows zero up to `padded`; SCALED: row n times its factor (0 selects 0).
 // 16 bytes a lane on both sides; the tile of 8 x 8 chunks lies in LDS with chunk c of row r at c ^ (r / E), so that a column is read from all banks.
-template <class T>
+template <class T, bool SCALED>
 __global__ __launch_bounds__(256) void transpose_kernel(const T* src, int64_t src_pitch, int64_t rows, int64_t cols, T* dst, int64_t dst_pitch, int64_t padded,
-                                                        const float* scale, bool wide) {
+                                                        Factors factors, bool wide) {
     constexpr int E = 16 / (int)sizeof(T), SIDE = 8 * E, CHUNKS = SIDE * 8;
     struct alignas(16) Chunk { T v[E]; };
     __shared__ Chunk tile[CHUNKS];
@@ -565,8 +693,8 @@ __global__ __launch_bounds__(256) void transpose_kernel(const T* src, int64_t sr
 #pragma unroll
                 for (int e = 0; e < E; ++e)
                     if (col + e < cols) v.v[e] = from[e];
-            if (scale) {
-                const float f = scale[row];
+            if constexpr (SCALED) {
+                const float f = factors.weight_row(row);
                 if (f != 1.f)
 #pragma unroll
                     for (int e = 0; e < E; ++e) v.v[e] = f == 0.f ? (T)0.f : (T)((float)v.v[e] * f);
@@ -594,14 +722,16 @@ __global__ __launch_bounds__(256) void copy_rows_kernel(const T* src, int64_t sr
 
 // the sums of all runs of k, in their order, times the row's factor; 4 columns a lane where rows are multiples of 4
 template <class T>
-__global__ __launch_bounds__(256) void hidden_grad_kernel(const float* sums, int splits, int64_t rows, int64_t width, const float* scale, T* out) {
-    const int64_t n = blockIdx.x;
-    const float f = scale[n];
+__global__ __launch_bounds__(256) void hidden_grad_kernel(const float* sums, int splits, int64_t rows, int64_t width, Factors factors, T* out) {
+    const int64_t n = blockIdx.x, run = rows * width;
+    const float f = factors.hidden(n);
+    const float* from = sums + n * width;
     if ((width & 3) == 0) {
         struct alignas(4 * sizeof(T)) Four { T v[4]; };
         for (int64_t c = (int64_t)threadIdx.x * 4; c < width; c += 1024) {
             f32x4 v = {0.f, 0.f, 0.f, 0.f};
-            for (int s = 0; s < splits; ++s) v += *(const f32x4*)(sums + ((int64_t)s * rows + n) * width + c);
+#pragma unroll 8
+            for (int s = 0; s < splits; ++s) v += *(const f32x4*)(from + s * run + c);
             Four to;
 #pragma unroll
             for (int e = 0; e < 4; ++e) to.v[e] = (T)(f == 0.f ? 0.f : v[e] * f);
@@ -611,7 +741,8 @@ __global__ __launch_bounds__(256) void hidden_grad_kernel(const float* sums, int
     }
     for (int64_t c = threadIdx.x; c < width; c += 256) {
         float v = 0.f;
-        for (int s = 0; s < splits; ++s) v += sums[((int64_t)s * rows + n) * width + c];
+#pragma unroll 8
+        for (int s = 0; s < splits; ++s) v += from[s * run + c];
         out[n * width + c] = (T)(f == 0.f ? 0.f : v * f);
     }
 }
@@ -721,12 +852,12 @@ template <class T>
 void copy_rows(hipStream_t st, const void* src, int64_t pitch, int64_t rows, int64_t cols, void* dst, int64_t dst_pitch_bytes) {
     copy_rows_kernel<T><<<dim3((unsigned)rows), 256, 0, st>>>((const T*)src, pitch, cols, (T*)dst, dst_pitch_bytes / (int64_t)sizeof(T));
 }
-template <class T>
-void transpose(hipStream_t st, const void* src, int64_t pitch, int64_t rows, int64_t cols, void* dst, int64_t dst_pitch, int64_t padded, const float* scale) {
+template <class T, bool SCALED>
+void transpose(hipStream_t st, const void* src, int64_t pitch, int64_t rows, int64_t cols, void* dst, int64_t dst_pitch, int64_t padded, const Factors& factors) {
     constexpr int SIDE = 128 / (int)sizeof(T);
     const bool wide = ((uintptr_t)src & 15) == 0 && pitch * (int64_t)sizeof(T) % 16 == 0;
-    transpose_kernel<T><<<dim3((unsigned)((padded + SIDE - 1) / SIDE), (unsigned)((cols + SIDE - 1) / SIDE)), 256, 0, st>>>((const T*)src, pitch, rows, cols, (T*)dst, dst_pitch,
-                                                                                                                           padded, scale, wide);
+    transpose_kernel<T, SCALED><<<dim3((unsigned)((padded + SIDE - 1) / SIDE), (unsigned)((cols + SIDE - 1) / SIDE)), 256, 0, st>>>((const T*)src, pitch, rows, cols, (T*)dst,
+                                                                                                                                   dst_pitch, padded, factors, wide);
 }
 
 int check_head(const cs_head_loss* h) {
@@ -755,12 +886,11 @@ int forward(const cs_head_loss& h, const Plan& p, const Saved& s, float* row_los
     const int size = sizeof(T);
     const bool kd = h.kind == CS_HEAD_DISTILLATION;
     if (h.rows) {
+        const Targets targets{h.ids, h.ids_bits, h.ids_pitch, h.ignore_index};
         if (kd) {
             const int threads = h.top <= 64 ? 64 : h.top <= 128 ? 128 : 256;
             teacher_rows_kernel<<<dim3((unsigned)h.rows), threads, 0, st>>>(h.ids, h.ids_bits, h.ids_pitch, h.teacher, h.teacher_type, h.teacher_pitch, h.top, h.vocab,
                                                                            1.0 / h.temperature, p.entropy, s);
-        } else {
-            target_rows_kernel<<<dim3((unsigned)((h.rows + 255) / 256)), 256, 0, st>>>(h.ids, h.ids_bits, h.ids_pitch, h.rows, h.vocab, h.ignore_index, s);
         }
         if (p.hidden) copy_rows<T>(st, h.hidden, h.hidden_pitch, h.rows, h.width, p.hidden, p.hidden_pitch);
         if (p.weight) copy_rows<T>(st, h.weight, h.weight_pitch, h.vocab, h.width, p.weight, p.weight_pitch);
@@ -770,10 +900,23 @@ int forward(const cs_head_loss& h, const Plan& p, const Saved& s, float* row_los
         const Shape sh = shape_for(h.vocab, h.rows);
         const int tiles = (int)((h.vocab + SHAPES[sh].m - 1) / SHAPES[sh].m);
         const Cut whole{1, (kbytes + 127) / 128};
-        if (int rc = kd ? launch_product<KIND>(st, sh, a, b, kbytes, whole, NormEpi<true>{p.part, s, (int)h.rows, (int)h.vocab, h.top, c})
-                        : launch_product<KIND>(st, sh, a, b, kbytes, whole, NormEpi<false>{p.part, s, (int)h.rows, (int)h.vocab, h.top, c}))
+        if (int rc = kd ? launch_product<KIND>(st, sh, a, b, kbytes, whole, NormEpi<true>{p.part, s, targets, (int)h.rows, (int)h.vocab, h.top, c})
+                        : launch_product<KIND>(st, sh, a, b, kbytes, whole, NormEpi<false>{p.part, s, targets, (int)h.rows, (int)h.vocab, h.top, c}))
             return rc;
-        row_loss_kernel<<<dim3((unsigned)((h.rows + 3) / 4)), 256, 0, st>>>(p.part, tiles, h.rows, h.top, kd, c, h.temperature, p.entropy, s, p.losses, row_losses);
+        const bool mean = h.reduction == CS_REDUCE_MEAN;
+        if (h.rows <= FEW_ROWS) {
+            if (kd) few_losses_kernel<true><<<1, 1024, 0, st>>>(p.part, tiles, (int)h.rows, h.top, h.vocab, c, h.temperature, p.entropy, targets, s, row_losses, mean, loss, s.inv_count);
+            else few_losses_kernel<false><<<1, 1024, 0, st>>>(p.part, tiles, (int)h.rows, h.top, h.vocab, c, h.temperature, p.entropy, targets, s, row_losses, mean, loss, s.inv_count);
+            CS_HIP(hipGetLastError());
+            return CS_OK;
+        }
+        const dim3 grid((unsigned)((h.rows + 3) / 4));
+        if (kd) row_loss_kernel<true><<<grid, 256, 0, st>>>(p.part, tiles, h.rows, h.top, h.vocab, c, h.temperature, p.entropy, targets, s, p.losses, row_losses);
+        else row_loss_kernel<false><<<grid, 256, 0, st>>>(p.part, tiles, h.rows, h.top, h.vocab, c, h.temperature, p.entropy, targets, s, p.losses, row_losses);
+        if (h.reduction == CS_REDUCE_NONE) {                             // nothing to reduce: the backward pass has a gradient per row
+            CS_HIP(hipGetLastError());
+            return CS_OK;
+        }
     }
     reduce_loss_kernel<<<1, 1024, 0, st>>>(p.losses, s.state, h.rows, h.reduction == CS_REDUCE_MEAN, loss, s.inv_count);
     CS_HIP(hipGetLastError());
@@ -791,12 +934,15 @@ int backward(const cs_head_loss& h, const Plan& p, const Saved& s, const float* 
     }
     const bool kd = h.kind == CS_HEAD_DISTILLATION;
     const float c = (float)(1.4426950408889634 / h.temperature);
-    row_scale_kernel<<<1, 1024, 0, st>>>(grad, grad_stride, h.reduction == CS_REDUCE_NONE, s.state, s.inv_count, h.rows, (float)h.temperature, 1.f / Elem<KIND>::G_SCALE,
-                                         p.to_h, p.in_w, p.w_scale);
+    Factors factors{grad, s.inv_count, s.state, nullptr, nullptr, nullptr, (float)(h.temperature / (double)Elem<KIND>::G_SCALE)};
+    if (h.reduction == CS_REDUCE_NONE) {
+        row_scale_kernel<<<1, 1024, 0, st>>>(grad, grad_stride, s.state, h.rows, factors.f, p.to_h, p.in_w, p.w_scale);
+        factors.to_h = p.to_h, factors.in_w = p.in_w, factors.w_scale = p.w_scale;
+    }
     if (p.hidden) copy_rows<T>(st, h.hidden, h.hidden_pitch, h.rows, h.width, p.hidden, p.hidden_pitch);
     if (p.weight) copy_rows<T>(st, h.weight, h.weight_pitch, h.vocab, h.width, p.weight, p.weight_pitch);
     const int kbytes = (int)(p.hidden || p.weight ? up(h.width * size, 16) : h.width * size);
-    if (gw) transpose<T>(st, h.hidden, h.hidden_pitch, h.rows, h.width, p.ht, p.row_pitch, up(h.rows, 32), p.in_w);
+    if (gw) transpose<T, true>(st, h.hidden, h.hidden_pitch, h.rows, h.width, p.ht, p.row_pitch, up(h.rows, 32), factors);
     for (int64_t from = 0; from < h.vocab; from += p.piece) {
         const int64_t len = h.vocab - from < p.piece ? h.vocab - from : p.piece, klen = up(len, 64);
         const Operand a{(p.weight ? p.weight : (const char*)h.weight) + from * p.weight_pitch, p.weight_pitch, len};
@@ -809,7 +955,7 @@ int backward(const cs_head_loss& h, const Plan& p, const Saved& s, const float* 
                         : launch_product<KIND>(st, sh, a, b, kbytes, whole, GradEpi<KIND, false>{g, gt, p.piece_pitch, p.row_pitch, s, (int)h.rows, (int)from, (int)len, h.top, c}))
             return rc;
         if (gh) {
-            transpose<T>(st, (const T*)h.weight + from * h.weight_pitch, h.weight_pitch, len, h.width, p.wt, p.piece_pitch, klen, nullptr);
+            transpose<T, false>(st, (const T*)h.weight + from * h.weight_pitch, h.weight_pitch, len, h.width, p.wt, p.piece_pitch, klen, factors);
             const int kb = (int)(klen * size), slabs = (kb + 127) / 128;
             const Cut cut{(slabs + p.cut.per - 1) / p.cut.per, p.cut.per};
             const SumEpi epi{p.sums, (int)h.rows, (int)h.width, from != 0};
@@ -817,13 +963,13 @@ int backward(const cs_head_loss& h, const Plan& p, const Saved& s, const float* 
         }
         if (gw) {
             const int kb = (int)(up(h.rows, 32) * size);
-            const OutEpi<KIND> epi{(T*)gw + from * h.width, (int)len, (int)h.width, p.w_scale};
+            const OutEpi<KIND> epi{(T*)gw + from * h.width, (int)len, (int)h.width, factors};
             if (int rc = launch_product<KIND>(st, shape_for(h.width, len), Operand{p.ht, p.row_pitch * size, h.width}, Operand{p.gt, p.row_pitch * size, len}, kb,
                                               Cut{1, (kb + 127) / 128}, epi))
                 return rc;
         }
     }
-    if (gh) hidden_grad_kernel<T><<<dim3((unsigned)h.rows), 256, 0, st>>>(p.sums, p.cut.splits, h.rows, h.width, p.to_h, (T*)gh);
+    if (gh) hidden_grad_kernel<T><<<dim3((unsigned)h.rows), 256, 0, st>>>(p.sums, p.cut.splits, h.rows, h.width, factors, (T*)gh);
     CS_HIP(hipGetLastError());
     return CS_OK;
 }

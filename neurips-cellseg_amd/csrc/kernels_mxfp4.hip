@@ -149,8 +149,9 @@ struct LinearEpi {
     T* out;            // [rows][outputs]
     int rows, outputs;
     template <class R> static constexpr int lds() { return stage_bytes<R, T>(); }
+    template <class R> __device__ __forceinline__ NoAhead ahead(Tile, int) const { return {}; }
     template <class R>
-    __device__ __forceinline__ void operator()(const Problem& p, Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF]) const {
+    __device__ __forceinline__ void operator()(const Problem& p, Tile t, char* lds, f32x4 (&acc)[R::MF][R::NF], NoAhead) const {
         store_tile<R>(t, lds, acc, out, outputs, rows, outputs, false, [](float v) { return v; });
     }
 };

@@ -389,6 +389,7 @@ typedef struct cs_head_loss {
     int ids_bits;               /* 32 or 64 */
     int teacher_type;           /* CS_TYPE_* */
     int top;                    /* distillation; the cross entropy takes 1 */
+    int keep_scores;            /* 1: for gradients of up to 64 rows the forward pass keeps their z, where they take no more than the weight; the same in all calls */
 } cs_head_loss;
 size_t cs_head_loss_saved_bytes(const cs_head_loss* head_host);
 /* backward: 0 the forward pass; else the backward pass with the gradients wanted (bit 0: hidden, bit 1: weight) */

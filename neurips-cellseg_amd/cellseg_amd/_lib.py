@@ -40,7 +40,7 @@ class HeadLoss(C.Structure):
     _fields_ = ([(n, C.c_void_p) for n in ("hidden", "weight", "ids", "teacher")]
                 + [(n, C.c_int64) for n in ("hidden_pitch", "weight_pitch", "ids_pitch", "teacher_pitch", "rows", "vocab", "width", "ignore_index")]
                 + [("temperature", C.c_double)]
-                + [(n, C.c_int) for n in ("type", "kind", "reduction", "ids_bits", "teacher_type", "top")])
+                + [(n, C.c_int) for n in ("type", "kind", "reduction", "ids_bits", "teacher_type", "top", "keep_scores")])
 
 
 class SwiPlan(C.Structure):

@@ -136,6 +136,7 @@ class _HeadLoss(torch.autograd.Function):
     def forward(ctx, hidden, weight, ids, teacher, kind, reduction, ignore_index, temperature):
         top = 1 if teacher is None else ids.shape[1]
         head = _descriptor(hidden, weight, kind, reduction, ignore_index, temperature, top, ids, teacher)
+        head.keep_scores = int(ctx.needs_input_grad[0] or ctx.needs_input_grad[1])
         with torch.cuda.device(hidden.device):
             size = lib.cs_head_loss_saved_bytes(head)
             if not size:

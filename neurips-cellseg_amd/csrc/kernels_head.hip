@@ -16,6 +16,7 @@ using namespace nt;
 
 constexpr int KD_MAX_TOP = 1024;
 constexpr int NO_ID = 0x7fffffff;
+constexpr int FEW_ROWS = 64;
 enum RowState { ROW_SKIP = 0, ROW_COUNT = 1, ROW_BAD = 2 };
 
 template <int KIND> struct Elem;
@@ -34,6 +35,7 @@ struct Saved {
     float* z;          // [rows][top]
     uint16_t* starts;  // [rows][starts_pitch] distillation: how many ids of the row lie below 128 t
     int64_t starts_pitch;
+    float* scores;     // up to FEW_ROWS rows: z of the whole vocabulary, 1 KB a run of 32 ids and 16 rows: lane l's ids run + 4 (l / 16) + {0..3, 16..19}, row l % 16; else NULL
 };
 
 __device__ __forceinline__ int64_t id_at(const void* ids, int bits, int64_t i) {
@@ -111,6 +113,14 @@ struct NormEpi {
             hold<R>(acc, j);
 #pragma unroll
             for (int i = 0; i < R::MF; ++i) v[i] = take(acc[i][j]);
+            if constexpr (R::TILE_N == 32) {                             // few rows: a lane holds what one of their gradients' products takes
+                const int block = (n0 + R::col0(wn, j)) >> 4, blocks = (rows + 15) >> 4;
+                if (s.scores && block < blocks) {
+                    float* const to = s.scores + ((((int64_t)m0 + R::row0(wm, 0)) >> 5) * blocks + block) * 512 + lane * 8;
+                    *(f32x4*)to = v[0];
+                    *(f32x4*)(to + 4) = v[1];
+                }
+            }
             float m = -INFINITY, sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < R::MF; ++i)
@@ -378,11 +388,20 @@ enum Shape { LARGE, MIDDLE, FLAT };
 struct ShapeSize { int m, n; };
 constexpr ShapeSize SHAPES[3] = {{256, 256}, {128, 128}, {128, 32}};
 
-// splits: into how many runs of k the product may be cut
-Shape shape_for(int64_t m, int64_t n, int64_t splits = 1) {
-    const int64_t large = ((m + 255) / 256) * ((n + 255) / 256);
+// Rounds over the 256 CUs, in units of a middle tile's products at full rate.  A large tile runs at that rate; fp32 middle tiles at 0.87 of it, two
+// on a CU or one, 16-bit ones at 0.7 and, alone on their CU, at 0.53 (16384 x 4096 with 65..1000 rows: a large tile 943 / 104 us, middle tiles 278 / 50
+// us for one on each CU, 536 / 73 us for two).  So 100 rows of a large vocabulary, which leave most of a 256 x 256 tile empty, go to middle
+// tiles and 200 go to large ones.  splits: into how many runs of 32 slabs k may be cut, 8 times as many for middle tiles.
+Shape shape_for(int64_t m, int64_t n, int size, int64_t splits = 1) {
     if (n <= 64) return FLAT;
-    return large * (splits > 1 ? splits : 1) >= 192 ? LARGE : MIDDLE;
+    const int64_t tl = ((m + 255) / 256) * ((n + 255) / 256), tm = ((m + 127) / 128) * ((n + 127) / 128);
+    int64_t sl = 1, sm = 1;
+    if (splits > 1) {
+        sl = tl >= 192 ? 1 : CUS / tl < splits ? CUS / tl : splits;
+        sm = tm >= 256 ? 1 : (512 + tm - 1) / tm < splits * 8 ? (512 + tm - 1) / tm : splits * 8;
+    }
+    const double large = 4.0 * (double)((tl * sl + CUS - 1) / CUS) / (double)sl, rounds = (double)((tm * sm + CUS - 1) / CUS) / (double)sm;
+    return large <= rounds * (size == 4 ? 1.15 : tm * sm <= CUS ? 1.9 : 1.4) ? LARGE : MIDDLE;
 }
 
 struct Cut { int splits, per; };
@@ -634,7 +653,6 @@ __global__ __launch_bounds__(1024) void reduce_loss_kernel(const double* losses,
 }
 
 // both for few rows, in one launch of one block
-constexpr int FEW_ROWS = 64;
 template <bool LIST>
 __global__ __launch_bounds__(1024) void few_losses_kernel(const float2* part, int tiles, int rows, int top, int64_t vocab, float c, double t, const double* entropy,
                                                           Targets targets, Saved s, float* out, bool mean, float* loss, float* inv_count) {
@@ -752,6 +770,259 @@ __global__ __launch_bounds__(256) void zero_kernel(T* out, int64_t n) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) out[i] = (T)0.f;
 }
 
+// ---- the gradients of few rows -------------------------------------------------------------------------------------------------------------
+// Up to 64 rows are bound by the weight's bytes: the forward pass keeps z (no more bytes than the weight), and the weight is read, and its gradient
+// written, once more: no transposes, no second product.  G = p - q, kept as the sum of two 16-bit values (with few rows the rounding of one would
+// be the largest of the gradient's errors: nothing averages it), costs two instructions where one would do, which the memory hides.
+// The order of k inside an instruction is free as long as both operands share it:
+//   dH[n][d] = sum_v G[n][v] W[v][d]   k-slot (lane / 16, e) is id 4 (lane / 16) + e, e < 4, and 16 + 4 (lane / 16) + e - 4 of a run of 32 ids: what
+//                                      a lane holds of z
+//   dW[v][d] = sum_n G[v][n] H[n][d]   k-slot (lane / 16, e) is row 8 (lane / 16) + e of a run of 32
+// W and H come straight from memory, 16 bytes of 8 rows a lane, and are turned in registers into one operand per column.
+// A piece (1 KB twice) holds, per lane, 8 values: 16 bits: the high parts, the low parts; fp32: four and four.
+template <int KIND>
+__device__ __forceinline__ void put_piece(char* to, int lane, const float (&v)[8]) {
+    typedef typename Elem<KIND>::T T;
+    if constexpr (sizeof(T) == 2) {
+        struct alignas(16) Chunk { T v[8]; } high, low;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            high.v[e] = (T)v[e];
+            low.v[e] = (T)(v[e] - (float)high.v[e]);
+        }
+        *(Chunk*)(to + lane * 16) = high;
+        *(Chunk*)(to + 1024 + lane * 16) = low;
+    } else {
+        *(f32x4*)(to + lane * 16) = f32x4{v[0], v[1], v[2], v[3]};
+        *(f32x4*)(to + 1024 + lane * 16) = f32x4{v[4], v[5], v[6], v[7]};
+    }
+}
+
+// z -> pieces of G for dH, [run of 32 ids][16 rows], and, times the row's factor, for dW, [run of 32 ids][32 rows][16 ids].  A wave takes a run.
+template <int KIND, bool LIST>
+__global__ __launch_bounds__(256) void few_scores_kernel(Saved s, Factors factors, int rows, int64_t from, int64_t runs, int top, float c, char* g_h, char* g_w) {
+    __shared__ float turn[4][32 * 36];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, col = lane & 15, blocks = (rows + 15) >> 4;
+    const int64_t run = (int64_t)blockIdx.x * 4 + wave;
+    if (run >= runs) return;
+    const int64_t id0 = from + run * 32;
+    float* const mine = turn[wave];
+    for (int b32 = 0; b32 * 2 < blocks; ++b32) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int block = b32 * 2 + j, n = block * 16 + col, in = min(n, rows - 1);
+            float v[8] = {};
+            if (block < blocks) {
+                const float* z = s.scores + ((from >> 5) + run) * blocks * 512 + block * 512 + lane * 8;
+                const f32x4 z0 = *(const f32x4*)z, z1 = *(const f32x4*)(z + 4);
+                const float2 norm = s.norm[in];
+                const int state = n < rows ? s.state[in] : ROW_SKIP;
+                const float inv = state == ROW_BAD ? __builtin_nanf("") : norm.y;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = __builtin_amdgcn_exp2f(fmaf(e < 4 ? z0[e & 3] : z1[e & 3], c, -norm.x)) * inv;
+                int2 at = make_int2(0, 1);
+                if constexpr (LIST) at = listed_of(s, in, (int)(id0 & ~(int64_t)127), 128);
+                if (state != ROW_COUNT) at.y = at.x;
+                for (int e = at.x; e < at.y; ++e) {
+                    const int64_t entry = (int64_t)in * top + e;
+                    const int want = s.ids[entry] - (int)id0;
+                    const float target = LIST ? s.q[entry] : 1.f;
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) v[x] -= want == (x < 4 ? 0 : 12) + 4 * q + x ? target : 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = state == ROW_SKIP ? 0.f : v[e] * Elem<KIND>::G_SCALE;
+                if (g_h) put_piece<KIND>(g_h + (run * blocks + block) * 2048, lane, v);
+                const float f = n < rows ? factors.weight_row(n) : 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = f == 0.f ? 0.f : v[e] * f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mine[((e < 4 ? 0 : 12) + 4 * q + e) * 36 + j * 16 + col] = v[e];
+        }
+        wave_sync();
+        if (g_w)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const f32x4 a = *(const f32x4*)(mine + (i * 16 + col) * 36 + q * 8), b = *(const f32x4*)(mine + (i * 16 + col) * 36 + q * 8 + 4);
+                const float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+                put_piece<KIND>(g_w + ((run * ((blocks + 1) >> 1) + b32) * 2 + i) * 2048, lane, v);
+            }
+        wave_sync();
+    }
+}
+
+// 8 rows of 16 bytes -> one operand of 8 values per column
+template <int KIND> struct Turned;
+template <int KIND>
+struct Turned16 {
+    static constexpr int COLS = 8;
+    i32x4 v[8];
+    __device__ __forceinline__ void set(const i32x4 (&r)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[j][e] = (int)__builtin_amdgcn_perm((unsigned)r[2 * e + 1][j >> 1], (unsigned)r[2 * e][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+    }
+    // sum += (high + low) x column j
+    __device__ __forceinline__ f32x4 times(i32x4 high, i32x4 low, int j, f32x4 sum) const {
+        return mma<KIND, 0>(low, v[j], mma<KIND, 0>(high, v[j], sum, 0, 0), 0, 0);
+    }
+};
+template <> struct Turned<BF16> : Turned16<BF16> {};
+template <> struct Turned<FP16> : Turned16<FP16> {};
+template <>
+struct Turned<FP32> {
+    static constexpr int COLS = 4;
+    i32x4 v[8];
+    __device__ __forceinline__ void set(const i32x4 (&r)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = r[e];
+    }
+    __device__ __forceinline__ f32x4 times(i32x4 a, i32x4 b, int j, f32x4 sum) const {
+        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = __builtin_amdgcn_mfma_f32_16x16x4f32(e < 4 ? x[e & 3] : y[e & 3], __builtin_bit_cast(f32x4, v[e])[j], sum, 0, 0, 0);
+        return sum;
+    }
+};
+
+typedef i32x4 Loose __attribute__((aligned(2)));                         // 16 bytes at the address of any value
+typedef f32x4 LooseSum __attribute__((aligned(4)));
+
+struct FewGrads {
+    const char *hidden, *weight;           // of the first id here
+    int64_t hidden_pitch, weight_pitch;    // bytes, any
+    const char *g_h, *g_w;                 // pieces, NULL where that gradient is not wanted
+    float* sums;                           // [splits][rows][width] of dH
+    char* out;                             // dW of the first id here, rows of `width`
+    int rows, width, groups, splits;
+    int64_t ids, runs, runs_per_split;
+    bool add;
+    Factors factors;
+};
+
+// A wave takes 16 bytes of 16 lanes = 256 bytes of columns and a run of ids; the four waves of a block lie side by side and share G in the caches,
+// the blocks of one run of ids lie in one XCD.  Behind the last column a lane computes the last whole 16 bytes again and stores the same values.
+template <int KIND, int BLOCKS>
+__global__ __launch_bounds__(256, BLOCKS == 1 ? 2 : 1) void few_grads_kernel(FewGrads p) {
+    typedef typename Elem<KIND>::T T;
+    typedef Turned<KIND> Op;
+    constexpr int COLS = Op::COLS, PAIRS = (BLOCKS + 1) / 2;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, col = lane & 15;
+    const int id = blockIdx.x, split = (id / (8 * p.groups)) * 8 + id % 8, chunk = (id / 8 % p.groups) * 4 + wave;
+    if (split >= p.splits || chunk * 16 * COLS >= p.width) return;
+    const int d = min((chunk * 16 + col) * COLS, p.width - COLS);
+    const int64_t first = split * p.runs_per_split, last = min(first + p.runs_per_split, p.runs) - 1;
+    Op h[PAIRS];
+    if (p.g_w) {
+#pragma unroll
+        for (int k = 0; k < PAIRS; ++k) {
+            i32x4 r[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int n = k * 32 + q * 8 + e, in = min(n, p.rows - 1);
+                const bool counts = p.factors.in_w ? p.factors.in_w[in] != 0.f : p.factors.state[in] != ROW_SKIP;
+                const int keep = n < p.rows && counts ? ~0 : 0;
+                r[e] = *(const Loose*)(p.hidden + in * p.hidden_pitch + (int64_t)d * sizeof(T)) & i32x4{keep, keep, keep, keep};
+            }
+            h[k].set(r);
+        }
+    }
+    f32x4 sum[BLOCKS][COLS];
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+        for (int j = 0; j < COLS; ++j) sum[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const float f = p.g_w ? p.factors.weight() : 0.f;
+    i32x4 next[8];
+    auto load = [&](int64_t run) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int64_t v = min(run * 32 + (e < 4 ? 0 : 12) + 4 * q + e, p.ids - 1);
+            next[e] = *(const Loose*)(p.weight + v * p.weight_pitch + (int64_t)d * sizeof(T));
+        }
+    };
+    if (p.g_h) load(first);
+#pragma unroll 1
+    for (int64_t run = first; run <= last; ++run) {
+        i32x4 gh[BLOCKS][2], gw[PAIRS][2][2];
+        if (p.g_w)
+#pragma unroll
+            for (int k = 0; k < PAIRS; ++k)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) gw[k][i][x] = *(const i32x4*)(p.g_w + ((run * PAIRS + k) * 2 + i) * 2048 + x * 1024 + lane * 16);
+        if (p.g_h) {
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) gh[b][x] = *(const i32x4*)(p.g_h + (run * BLOCKS + b) * 2048 + x * 1024 + lane * 16);
+            Op w;
+            w.set(next);
+            load(min(run + 1, last));
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+                for (int j = 0; j < COLS; ++j) sum[b][j] = w.times(gh[b][0], gh[b][1], j, sum[b][j]);
+        }
+        if (p.g_w)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                f32x4 dw[COLS];
+#pragma unroll
+                for (int j = 0; j < COLS; ++j) {
+                    dw[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < PAIRS; ++k) dw[j] = h[k].times(gw[k][i][0], gw[k][i][1], j, dw[j]);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    struct alignas(16) Chunk { T v[COLS]; } to;
+#pragma unroll
+                    for (int j = 0; j < COLS; ++j) to.v[j] = (T)(dw[j][r] * f);
+                    const int64_t v = run * 32 + i * 16 + q * 4 + r;
+                    if (v < p.ids) __builtin_nontemporal_store(__builtin_bit_cast(i32x4, to), (Loose*)(p.out + (v * p.width + d) * (int64_t)sizeof(T)));
+                }
+            }
+    }
+    if (!p.g_h) return;
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int n = b * 16 + q * 4 + r;
+            if (n >= p.rows) continue;
+            float* to = p.sums + ((int64_t)split * p.rows + n) * p.width + d;
+#pragma unroll
+            for (int j = 0; j < COLS; j += 4) {
+                f32x4 v = {sum[b][j][r], sum[b][j + 1][r], sum[b][j + 2][r], sum[b][j + 3][r]};
+                if (p.add) v += *(const LooseSum*)(to + j);
+                *(LooseSum*)(to + j) = v;
+            }
+        }
+}
+
+// the sums of all runs of ids, 16 waves a block, 64 columns of a row
+template <class T>
+__global__ __launch_bounds__(1024) void few_hidden_kernel(const float* sums, int splits, int64_t rows, int64_t width, Factors factors, T* out) {
+    __shared__ float part[16][64];
+    const int64_t n = blockIdx.y, c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63), run = rows * width;
+    const int group = threadIdx.x >> 6;
+    float v = 0.f;
+    if (c < width)
+#pragma unroll 4
+        for (int s = group; s < splits; s += 16) v += sums[s * run + n * width + c];
+    part[group][threadIdx.x & 63] = v;
+    __syncthreads();
+    if (group || c >= width) return;
+#pragma unroll
+    for (int g = 1; g < 16; ++g) v += part[g][threadIdx.x];
+    const float f = factors.hidden(n);
+    out[n * width + c] = (T)(f == 0.f ? 0.f : v * f);
+}
+
 // ---- host -----------------------------------------------------------------------------------------------------------------------------
 struct Arena {
     char* base;
@@ -764,6 +1035,12 @@ struct Arena {
 };
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 int type_bytes(int type) { return type == CS_TYPE_FP32 ? 4 : 2; }
+
+// whether the forward pass keeps z and few_grads_kernel makes the gradients: few rows, and z takes no more than the weight
+bool few(const cs_head_loss& h) {
+    const int size = type_bytes(h.type);
+    return h.keep_scores && h.rows && h.rows <= FEW_ROWS && h.width * size >= 16 && up(h.rows, 16) * 4 <= h.width * size;
+}
 
 Saved carve_saved(const cs_head_loss& h, void* base, size_t* bytes) {
     Arena a{(char*)base};
@@ -779,6 +1056,7 @@ Saved carve_saved(const cs_head_loss& h, void* base, size_t* bytes) {
     s.starts_pitch = (h.vocab + 255) / 256 * 2 + 1;
     s.starts = a.take<uint16_t>(kd ? n * (size_t)s.starts_pitch : 0);
     if (!kd) s.starts = nullptr;
+    s.scores = few(h) ? a.take<float>((size_t)(up(h.vocab, 128) * up(h.rows, 16))) : nullptr;
     *bytes = a.at;
     return s;
 }
@@ -802,6 +1080,8 @@ struct Plan {
     Shape dh_shape;
     char *g, *gt, *wt, *ht;
     float *sums, *to_h, *in_w, *w_scale;
+    int64_t runs, runs_per_split;          // few rows: of 32 ids, in a piece and for a block; blocks side by side and along the ids
+    int groups, splits;
 };
 
 constexpr int64_t PIECE_BYTES = (int64_t)512 << 20;      // of G
@@ -814,10 +1094,31 @@ Plan make_plan(const cs_head_loss& h, int backward, void* base) {
     const bool hin = in_place(h.hidden, h.hidden_pitch, h.width, size), win = in_place(h.weight, h.weight_pitch, h.width, size);
     p.hidden_pitch = hin ? h.hidden_pitch * size : width_pitch;
     p.weight_pitch = win ? h.weight_pitch * size : width_pitch;
+    if (backward && few(h)) {
+        const int64_t runs = up(h.vocab, 32) / 32, run_bytes = up(h.rows, 16) * 128, most = PIECE_BYTES / run_bytes / 4 * 4;
+        const int blocks = (int)(up(h.rows, 16) / 16);
+        p.runs = runs < most ? runs : most;
+        p.groups = (int)((h.width * size + 1023) / 1024);
+        const int64_t want = blocks == 1 ? 2 * CUS : CUS;                // blocks that run at a time; 4 runs of ids at least
+        int64_t splits = p.groups < want ? want / p.groups : 1;
+        if (splits > p.runs / 4) splits = p.runs / 4 > 0 ? p.runs / 4 : 1;
+        p.runs_per_split = (p.runs + splits - 1) / splits;
+        p.splits = (int)((p.runs + p.runs_per_split - 1) / p.runs_per_split);
+        p.to_h = a.take<float>((size_t)h.rows);
+        p.in_w = a.take<float>((size_t)h.rows);
+        p.w_scale = a.take<float>(1);
+        if (backward & 1) {
+            p.g = a.take<char>((size_t)(p.runs * run_bytes));
+            p.sums = a.take<float>((size_t)p.splits * h.rows * h.width);
+        }
+        if (backward & 2) p.gt = a.take<char>((size_t)(p.runs * up(h.rows, 32) * 128));
+        p.bytes = a.at;
+        return p;
+    }
     if (!hin) p.hidden = a.take<char>((size_t)(h.rows * width_pitch));
     if (!win) p.weight = a.take<char>((size_t)(h.vocab * width_pitch));
     if (!backward) {
-        const Shape sh = shape_for(h.vocab, h.rows);
+        const Shape sh = shape_for(h.vocab, h.rows, size);
         p.part = a.take<float2>((size_t)(h.rows * ((h.vocab + SHAPES[sh].m - 1) / SHAPES[sh].m)));
         p.losses = a.take<double>((size_t)h.rows);
         p.entropy = a.take<double>((size_t)(h.kind == CS_HEAD_DISTILLATION ? h.rows : 0));
@@ -834,7 +1135,7 @@ Plan make_plan(const cs_head_loss& h, int backward, void* base) {
         p.w_scale = a.take<float>(1);
         if (backward & 1) {
             const int kbytes = (int)((p.piece < h.vocab ? p.piece : up(h.vocab, 64)) * size);
-            p.dh_shape = shape_for(h.width, h.rows, kbytes / 128 / 32);  // runs of 32 slabs at least for large tiles
+            p.dh_shape = shape_for(h.width, h.rows, size, kbytes / 128 / 32);  // runs of 32 slabs at least for large tiles
             p.cut = cut_for(h.width, h.rows, kbytes, p.dh_shape, 64);
             p.wt = a.take<char>((size_t)(h.width * p.piece_pitch * size));
             p.sums = a.take<float>((size_t)p.cut.splits * h.rows * h.width);
@@ -897,7 +1198,7 @@ int forward(const cs_head_loss& h, const Plan& p, const Saved& s, float* row_los
         const Operand a{p.weight ? p.weight : (const char*)h.weight, p.weight_pitch, h.vocab}, b{p.hidden ? p.hidden : (const char*)h.hidden, p.hidden_pitch, h.rows};
         const int kbytes = (int)(p.hidden || p.weight ? up(h.width * size, 16) : h.width * size);
         const float c = (float)(1.4426950408889634 / h.temperature);
-        const Shape sh = shape_for(h.vocab, h.rows);
+        const Shape sh = shape_for(h.vocab, h.rows, size);
         const int tiles = (int)((h.vocab + SHAPES[sh].m - 1) / SHAPES[sh].m);
         const Cut whole{1, (kbytes + 127) / 128};
         if (int rc = kd ? launch_product<KIND>(st, sh, a, b, kbytes, whole, NormEpi<true>{p.part, s, targets, (int)h.rows, (int)h.vocab, h.top, c})
@@ -939,6 +1240,26 @@ int backward(const cs_head_loss& h, const Plan& p, const Saved& s, const float* 
         row_scale_kernel<<<1, 1024, 0, st>>>(grad, grad_stride, s.state, h.rows, factors.f, p.to_h, p.in_w, p.w_scale);
         factors.to_h = p.to_h, factors.in_w = p.in_w, factors.w_scale = p.w_scale;
     }
+    if (s.scores) {
+        for (int64_t from = 0; from < h.vocab; from += p.runs * 32) {
+            const int64_t len = h.vocab - from < p.runs * 32 ? h.vocab - from : p.runs * 32, runs = (len + 31) / 32;
+            const dim3 scores_grid((unsigned)((runs + 3) / 4));
+            char *const g_h = gh ? p.g : nullptr, *const g_w = gw ? p.gt : nullptr;
+            if (kd) few_scores_kernel<KIND, true><<<scores_grid, 256, 0, st>>>(s, factors, (int)h.rows, from, runs, h.top, c, g_h, g_w);
+            else few_scores_kernel<KIND, false><<<scores_grid, 256, 0, st>>>(s, factors, (int)h.rows, from, runs, h.top, c, g_h, g_w);
+            const FewGrads few{(const char*)h.hidden, (const char*)h.weight + from * h.weight_pitch * size, h.hidden_pitch * size, h.weight_pitch * size, g_h, g_w, p.sums,
+                               (char*)gw + from * h.width * size, (int)h.rows, (int)h.width, p.groups, (int)((runs + p.runs_per_split - 1) / p.runs_per_split), len, runs,
+                               p.runs_per_split, from != 0, factors};
+            const dim3 grid((unsigned)(up(few.splits, 8) * p.groups));
+            if (h.rows <= 16) few_grads_kernel<KIND, 1><<<grid, 256, 0, st>>>(few);
+            else if (h.rows <= 32) few_grads_kernel<KIND, 2><<<grid, 256, 0, st>>>(few);
+            else if (h.rows <= 48) few_grads_kernel<KIND, 3><<<grid, 256, 0, st>>>(few);
+            else few_grads_kernel<KIND, 4><<<grid, 256, 0, st>>>(few);
+        }
+        if (gh) few_hidden_kernel<T><<<dim3((unsigned)((h.width + 63) / 64), (unsigned)h.rows), 1024, 0, st>>>(p.sums, p.splits, h.rows, h.width, factors, (T*)gh);
+        CS_HIP(hipGetLastError());
+        return CS_OK;
+    }
     if (p.hidden) copy_rows<T>(st, h.hidden, h.hidden_pitch, h.rows, h.width, p.hidden, p.hidden_pitch);
     if (p.weight) copy_rows<T>(st, h.weight, h.weight_pitch, h.vocab, h.width, p.weight, p.weight_pitch);
     const int kbytes = (int)(p.hidden || p.weight ? up(h.width * size, 16) : h.width * size);
@@ -950,7 +1271,7 @@ int backward(const cs_head_loss& h, const Plan& p, const Saved& s, const float* 
         const Cut whole{1, (kbytes + 127) / 128};
         T* const g = (T*)p.g;
         T* const gt = gw ? (T*)p.gt : nullptr;
-        const Shape sh = shape_for(len, h.rows);
+        const Shape sh = shape_for(len, h.rows, size);
         if (int rc = kd ? launch_product<KIND>(st, sh, a, b, kbytes, whole, GradEpi<KIND, true>{g, gt, p.piece_pitch, p.row_pitch, s, (int)h.rows, (int)from, (int)len, h.top, c})
                         : launch_product<KIND>(st, sh, a, b, kbytes, whole, GradEpi<KIND, false>{g, gt, p.piece_pitch, p.row_pitch, s, (int)h.rows, (int)from, (int)len, h.top, c}))
             return rc;
@@ -964,7 +1285,7 @@ int backward(const cs_head_loss& h, const Plan& p, const Saved& s, const float* 
         if (gw) {
             const int kb = (int)(up(h.rows, 32) * size);
             const OutEpi<KIND> epi{(T*)gw + from * h.width, (int)len, (int)h.width, factors};
-            if (int rc = launch_product<KIND>(st, shape_for(h.width, len), Operand{p.ht, p.row_pitch * size, h.width}, Operand{p.gt, p.row_pitch * size, len}, kb,
+            if (int rc = launch_product<KIND>(st, shape_for(h.width, len, size), Operand{p.ht, p.row_pitch * size, h.width}, Operand{p.gt, p.row_pitch * size, len}, kb,
                                               Cut{1, (kb + 127) / 128}, epi))
                 return rc;
         }

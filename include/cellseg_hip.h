@@ -360,7 +360,8 @@ int cs_dice_ce_backward(const float* logits, const int64_t* logit_strides, const
 
 /* ------------------------------------------------------------------------------------------------
  * Losses of a linear head over a large vocabulary (no counterpart in the reference, whose loss has 3 classes).  z = hidden weight^T is
- * never held whole: the forward pass keeps per row its maximum and sum, the backward pass rebuilds z in pieces of the vocabulary.
+ * never held whole: the forward pass keeps per row its maximum and sum, the backward pass rebuilds z in pieces of the vocabulary.  (Up to 64
+ * rows, with keep_scores and where it takes no more than the weight, z is kept: `saved` is that much larger and the weight is read once less.)
  *   CS_HEAD_CROSS_ENTROPY  loss_i = lse(z_i) - z_i[target_i];  a row whose target is ignore_index has loss 0 and is not counted
  *   CS_HEAD_DISTILLATION   q_i = softmax(teacher_i / T) over the row's `top` entries, loss_i = T^2 sum_k q_ik (log q_ik - log p_i[id_ik]),
  *                          p_i = softmax(z_i / T) over the whole vocabulary.  An entry with a negative id or a teacher logit of -inf
@@ -371,7 +372,7 @@ int cs_dice_ce_backward(const float* logits, const int64_t* logit_strides, const
  * or length is not a multiple of 16 bytes are first copied into the workspace.  Sums, maxima and losses are held in 32 bits or more.
  * The backward pass needs the same descriptor, the `saved` bytes of its forward pass, and `grad` = d / d loss (device float; for
  * CS_REDUCE_NONE one per row, grad_stride floats apart); either gradient may be NULL.  Results do not depend on the launch order (no
- * atomics).  Gradients are contiguous and start at a multiple of 16 bytes.  Limits: 1 <= width < 2^21, 1 <= vocab < 2^30, 0 <= rows < 2^26, 1 <= top <= 1024, finite temperature > 0.
+ * atomics).  Gradients are contiguous and start at a multiple of 16 bytes.  Limits: 1 <= width < 2^21, 1 <= vocab < 2^30, 0 <= rows < 2^24, 1 <= top <= 1024, finite temperature > 0.
  * ---------------------------------------------------------------------------------------------- */
 enum { CS_TYPE_BF16 = 0, CS_TYPE_FP16 = 1, CS_TYPE_FP32 = 2 };
 enum { CS_HEAD_CROSS_ENTROPY = 0, CS_HEAD_DISTILLATION = 1 };
@@ -407,7 +408,7 @@ int cs_head_loss_backward(const cs_head_loss* head_host, const void* saved, size
  * with zeros.  A block that holds an infinity or a NaN has the scale 255, which reads as NaN.  x: `pitch` elements between rows, unit
  * inner stride.  cs_mxfp4_linear quantises x and multiplies it with quantised weights, y[r][o] = sum_k x[r][k] w[o][k] with fp32 sums
  * and one rounding to `type` (CS_TYPE_*, of x and y); y is contiguous.  No gradients.
- * Limits: 0 <= rows, outputs < 2^30, 1 <= width < 2^24; codes (linear: and y) start at a multiple of 4 (linear: 16) bytes.
+ * Limits: 0 <= rows, outputs < 2^30, 1 <= width < 2^24, and a linear layer that takes fewer than 2^24 thread blocks; codes (linear: and y) start at a multiple of 4 (linear: 16) bytes.
  * ---------------------------------------------------------------------------------------------- */
 int cs_mxfp4_quantize(const void* x, int64_t pitch, int64_t rows, int64_t width, int type, uint8_t* codes, uint8_t* scales, void* stream);
 int cs_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t width, int type, void* out, void* stream);

@@ -9,7 +9,11 @@ With rows i, vocabulary j, ``z = hidden weight^T``, ``p_i = softmax(z_i / T)``:
 
 ``hidden`` ``[..., D]`` and ``weight`` ``[V, D]`` share one type (bfloat16, float16 or float32) and get gradients of that type; products are
 summed, and losses returned, in float32.  16-bit gradients of the logits are rounded once to the type of the inputs before they are
-multiplied.  A float16 net wants the usual loss scale: a mean over many rows makes gradients smaller than float16 holds.
+multiplied (up to 64 rows they are kept as the sum of two 16-bit values).  For gradients of up to 64 rows the logits are kept where they take
+no more memory than the weight.  A float16 net wants the usual loss scale: a mean over many rows makes gradients smaller than float16 holds.
+
+Both directions can be captured into a graph; capture ``torch.autograd.grad``, as ``.backward()`` in a capture joins the stream on which an
+earlier, still living graph of the same leaves was built, which torch does not survive.
 """
 from __future__ import annotations
 

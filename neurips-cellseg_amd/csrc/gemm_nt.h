@@ -532,10 +532,11 @@ constexpr int CUS = 256;                     // of an MI355X: one block of large
 
 // Blocks of a launch.  Long tiles go to a block each: they are dealt out as CUs come free, and 1 % of a tile is saved by chaining them (16 tiles of
 // 64 slabs: 1.60 against 1.64 ms chained; 2 tiles of 510 slabs: 1.63 against 1.49 ms, the slowest CU's two).
+constexpr int64_t MOST_BLOCKS = (int64_t)1 << 24;      // of 256 threads in a launch, whose threads are counted in 32 bits: these excluded
 template <class R>
 unsigned grid_of(const Problem& p) {
     const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.splits;
-    return (unsigned)(Persistent<R>::value && p.slabs_per_split < 128 && tiles > CUS ? CUS : tiles);
+    return (unsigned)(Persistent<R>::value && (p.slabs_per_split < 128 || tiles >= MOST_BLOCKS) && tiles > CUS ? CUS : tiles);
 }
 
 }  // namespace nt

@@ -401,7 +401,7 @@ Shape shape_for(int64_t m, int64_t n, int size, int64_t splits = 1) {
         sm = tm >= 256 ? 1 : (512 + tm - 1) / tm < splits * 8 ? (512 + tm - 1) / tm : splits * 8;
     }
     const double large = 4.0 * (double)((tl * sl + CUS - 1) / CUS) / (double)sl, rounds = (double)((tm * sm + CUS - 1) / CUS) / (double)sm;
-    return large <= rounds * (size == 4 ? 1.15 : tm * sm <= CUS ? 1.9 : 1.4) ? LARGE : MIDDLE;
+    return tm >= MOST_BLOCKS || large <= rounds * (size == 4 ? 1.15 : tm * sm <= CUS ? 1.9 : 1.4) ? LARGE : MIDDLE;
 }
 
 struct Cut { int splits, per; };
@@ -420,7 +420,7 @@ Cut cut_for(int64_t m, int64_t n, int kbytes, Shape sh, int most) {
 template <int KIND, class EPI>
 int launch_product(hipStream_t st, Shape sh, const Operand& a, const Operand& b, int kbytes, Cut cut, const EPI& epi) {
     Problem p{a, b, kbytes, nullptr, nullptr, 0, 0, (int)((a.rows + SHAPES[sh].m - 1) / SHAPES[sh].m), (int)((b.rows + SHAPES[sh].n - 1) / SHAPES[sh].n), cut.splits, cut.per};
-    CS_REQUIRE((int64_t)p.tiles_m * p.tiles_n * p.splits < (int64_t)1 << 31, "head loss: too many tiles");
+    CS_REQUIRE((int64_t)p.tiles_m * p.tiles_n * p.splits < (sh == LARGE ? (int64_t)1 << 30 : MOST_BLOCKS), "head loss: too many tiles");
     if (sh == LARGE && p.kbytes % 128) product_kernel<Wide<KIND, true>, EPI><<<dim3(grid_of<Wide<KIND, true>>(p)), 256, 0, st>>>(p, epi);
     else if (sh == LARGE) product_kernel<Wide<KIND, false>, EPI><<<dim3(grid_of<Wide<KIND, false>>(p)), 256, 0, st>>>(p, epi);
     else if (sh == MIDDLE) product_kernel<Middle<KIND>, EPI><<<dim3(grid_of<Middle<KIND>>(p)), 256, 0, st>>>(p, epi);
@@ -734,8 +734,9 @@ __global__ __launch_bounds__(256) void transpose_kernel(const T* src, int64_t sr
 
 // src [rows][cols] -> dst [rows][pitch], zeros behind the columns
 template <class T>
-__global__ __launch_bounds__(256) void copy_rows_kernel(const T* src, int64_t src_pitch, int64_t cols, T* dst, int64_t pitch) {
-    for (int64_t c = threadIdx.x; c < pitch; c += 256) dst[(int64_t)blockIdx.x * pitch + c] = c < cols ? src[(int64_t)blockIdx.x * src_pitch + c] : (T)0.f;
+__global__ __launch_bounds__(256) void copy_rows_kernel(const T* src, int64_t src_pitch, int64_t rows, int64_t cols, T* dst, int64_t pitch) {
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
+        for (int64_t c = threadIdx.x; c < pitch; c += 256) dst[r * pitch + c] = c < cols ? src[r * src_pitch + c] : (T)0.f;
 }
 
 // the sums of all runs of k, in their order, times the row's factor; 4 columns a lane where rows are multiples of 4
@@ -1151,7 +1152,7 @@ Plan make_plan(const cs_head_loss& h, int backward, void* base) {
 
 template <class T>
 void copy_rows(hipStream_t st, const void* src, int64_t pitch, int64_t rows, int64_t cols, void* dst, int64_t dst_pitch_bytes) {
-    copy_rows_kernel<T><<<dim3((unsigned)rows), 256, 0, st>>>((const T*)src, pitch, cols, (T*)dst, dst_pitch_bytes / (int64_t)sizeof(T));
+    copy_rows_kernel<T><<<dim3((unsigned)(rows < (1 << 20) ? rows : 1 << 20)), 256, 0, st>>>((const T*)src, pitch, rows, cols, (T*)dst, dst_pitch_bytes / (int64_t)sizeof(T));
 }
 template <class T, bool SCALED>
 void transpose(hipStream_t st, const void* src, int64_t pitch, int64_t rows, int64_t cols, void* dst, int64_t dst_pitch, int64_t padded, const Factors& factors) {
@@ -1163,7 +1164,7 @@ void transpose(hipStream_t st, const void* src, int64_t pitch, int64_t rows, int
 
 int check_head(const cs_head_loss* h) {
     CS_REQUIRE(h, "head loss: NULL descriptor");
-    CS_REQUIRE(h->rows >= 0 && h->rows < (int64_t)1 << 26 && h->vocab >= 1 && h->vocab < (int64_t)1 << 30 && h->width >= 1 && h->width < (int64_t)1 << 21,
+    CS_REQUIRE(h->rows >= 0 && h->rows < MOST_BLOCKS && h->vocab >= 1 && h->vocab < (int64_t)1 << 30 && h->width >= 1 && h->width < (int64_t)1 << 21,
                "head loss: rows %lld, vocab %lld, width %lld out of range", (long long)h->rows, (long long)h->vocab, (long long)h->width);
     CS_REQUIRE(h->type >= CS_TYPE_BF16 && h->type <= CS_TYPE_FP32, "head loss: unknown type %d", h->type);
     CS_REQUIRE(h->kind == CS_HEAD_CROSS_ENTROPY || h->kind == CS_HEAD_DISTILLATION, "head loss: unknown kind %d", h->kind);

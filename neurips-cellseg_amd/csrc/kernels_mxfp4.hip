@@ -242,7 +242,7 @@ int launch_linear(hipStream_t st, Problem p, LinearEpi<T> epi) {
     p.tiles_n = (int)((p.b.rows + R::TILE_N - 1) / R::TILE_N);
     p.splits = 1;
     p.slabs_per_split = (p.kbytes + 127) / 128;
-    CS_REQUIRE((int64_t)p.tiles_m * p.tiles_n < (int64_t)1 << 31, "mxfp4 linear: too many tiles");
+    CS_REQUIRE((int64_t)p.tiles_m * p.tiles_n < (Persistent<R>::value ? (int64_t)1 << 30 : MOST_BLOCKS), "mxfp4 linear: too many tiles");
     linear_kernel<R, LinearEpi<T>><<<dim3(grid_of<R>(p)), R::THREADS, 0, st>>>(p, epi);
     CS_HIP(hipGetLastError());
     return CS_OK;
@@ -285,17 +285,27 @@ bool reads_wide(const void* x, int64_t pitch) {
     return ((uintptr_t)x & 15) == 0 && (pitch * (int64_t)sizeof(T)) % 16 == 0;
 }
 
+constexpr int64_t LAUNCH_ROWS = MOST_BLOCKS / 2;       // rows of a launch, a block each at most
+
 template <class T>
 int quantise(const void* x, int64_t pitch, int64_t rows, int64_t width, uint8_t* codes, uint8_t* scales, hipStream_t st) {
     const int64_t blocks = (width + 31) / 32;
-    quantise_kernel<T><<<row_blocks(rows, blocks * 4), 256, 0, st>>>((const T*)x, pitch, rows, width, (int)blocks, reads_wide<T>(x, pitch), codes, scales);
+    for (int64_t r = 0; r < rows; r += LAUNCH_ROWS) {
+        const int64_t some = rows - r < LAUNCH_ROWS ? rows - r : LAUNCH_ROWS;
+        quantise_kernel<T><<<row_blocks(some, blocks * 4), 256, 0, st>>>((const T*)x + r * pitch, pitch, some, width, (int)blocks, reads_wide<T>(x, pitch),
+                                                                       codes + r * blocks * 16, scales + r * blocks);
+    }
     CS_HIP(hipGetLastError());
     return CS_OK;
 }
 template <class T>
 int dequantise(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t width, void* out, hipStream_t st) {
     const int64_t blocks = (width + 31) / 32;
-    dequantise_kernel<T><<<row_blocks(rows, blocks * 4), 256, 0, st>>>(codes, scales, rows, width, (int)blocks, reads_wide<T>(out, width), (T*)out);
+    for (int64_t r = 0; r < rows; r += LAUNCH_ROWS) {
+        const int64_t some = rows - r < LAUNCH_ROWS ? rows - r : LAUNCH_ROWS;
+        dequantise_kernel<T><<<row_blocks(some, blocks * 4), 256, 0, st>>>(codes + r * blocks * 16, scales + r * blocks, some, width, (int)blocks, reads_wide<T>(out, width),
+                                                                         (T*)out + r * width);
+    }
     CS_HIP(hipGetLastError());
     return CS_OK;
 }
@@ -303,6 +313,7 @@ template <class T>
 int linear(const void* x, int64_t pitch, int64_t rows, int64_t width, const uint8_t* codes, const uint8_t* scales, int64_t outputs, void* y, const LinearPlan& p,
            hipStream_t st) {
     if (few_rows(rows, p.blocks)) {
+        CS_REQUIRE((outputs + 15) / 16 < MOST_BLOCKS, "mxfp4 linear: too many outputs");
         few_rows_kernel<T><<<dim3((unsigned)((outputs + 15) / 16)), 256, few_lds(rows, p.blocks), st>>>((const T*)x, pitch, (int)rows, width, (int)p.blocks,
                                                                                                    reads_wide<T>(x, pitch), codes, scales, (int)outputs, (T*)y);
         CS_HIP(hipGetLastError());
@@ -310,7 +321,7 @@ int linear(const void* x, int64_t pitch, int64_t rows, int64_t width, const uint
     }
     const int64_t padded = (p.blocks + 15) / 16 * 16;
     const int64_t x_blocks = row_blocks(p.rows_x, padded * 4), w_blocks = p.rows_w / 64 * (padded / 16);
-    CS_REQUIRE(x_blocks + w_blocks < (int64_t)1 << 31, "mxfp4 linear: too many outputs");
+    CS_REQUIRE(x_blocks + w_blocks < MOST_BLOCKS, "mxfp4 linear: too many outputs");
     prepare_kernel<T><<<dim3((unsigned)(x_blocks + w_blocks)), 256, 0, st>>>((const T*)x, pitch, rows, width, (int)p.blocks, reads_wide<T>(x, pitch), p.codes, p.scales_x,
                                                                              p.rows_x, scales, outputs, p.scales_w, p.rows_w, (unsigned)x_blocks);
     CS_HIP(hipGetLastError());

@@ -40,7 +40,8 @@ class Reference:
 
     def __init__(self, h, w, target=None, ids=None, logits=None, t=1.0, ignore=-100):
         dtype = h.dtype
-        self.u, self.tiny = unit(dtype), 2.0 ** -25 if dtype == torch.float16 else 0.0
+        self.ug = self.u = unit(dtype)                                   # of the inputs' type; of G, which few rows keep as the sum of two such numbers: u^2
+        self.tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
         self.h, self.w, self.t = h.double(), w.double(), t
         n, v = h.shape[0], w.shape[0]
         self.q = torch.zeros(n, v, dtype=torch.float64)
@@ -65,7 +66,7 @@ class Reference:
         """weight [rows]: d / d loss_i.  -> (dH, its bound, dW, its bound)"""
         f = (weight * self.live * self.t)[:, None]
         g = (self.p - self.q) * (f != 0)
-        eg = (self.p * (2 * self.ez + 2.0 ** -16) + self.q * 2.0 ** -23 + self.u * g.abs() + self.tiny * 2.0 ** -14) * (f != 0)
+        eg = (self.p * (2 * self.ez + 2.0 ** -16) + self.q * 2.0 ** -23 + self.ug * g.abs() + self.tiny * 2.0 ** -14) * (f != 0)
         dh, dw = f * (g @ self.w), (f * g).t() @ self.h
         n, v = g.shape
         bh = f.abs() * ((eg + (v + 64) * 2.0 ** -24 * g.abs()) @ self.w.abs()) + self.u * 1.01 * dh.abs() + 4 * 2.0 ** -24 * dh.abs() + self.tiny
@@ -374,3 +375,118 @@ def test_modules():
     a, b = h.to(DEV), w.to(DEV)
     assert torch.equal(ca.LinearCrossEntropyLoss(ignore_index=3, reduction="sum")(a, b, target.to(DEV)), ca.linear_cross_entropy(a, b, target.to(DEV), ignore_index=3, reduction="sum"))
     assert torch.equal(ca.LinearDistillationLoss(temperature=3.0)(a, b, ids.to(DEV), logits.to(DEV)), ca.linear_distillation(a, b, ids.to(DEV), logits.to(DEV), temperature=3.0))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("n,d", [(1, 130), (16, 77), (17, 257), (33, 300), (64, 515)])
+def test_few_rows_keep_more_of_the_gradient_and_read_any_address(n, d, kind):
+    """Up to 64 rows G keeps two roundings' worth of bits; rows of both matrices start at odd addresses; a row that does not count holds NaN."""
+    v, dtype = 2100, TYPES[kind]
+    h, w, target = make(n, v, d, dtype, seed=n + d)
+    if n > 1:
+        target[n // 2] = -100
+    ref = Reference(h, w, target)
+    ids, logits = teacher(n, v, 7)
+    ids[0] = -1
+    kd = Reference(h, w, ids=ids, logits=logits, t=2.0)
+    ref.ug = kd.ug = unit(dtype) ** 2 if kind != "fp32" else unit(dtype)
+    ids, logits, target = ids.to(DEV), logits.to(DEV), target.to(DEV)
+
+    def odd(x, off):
+        return torch.nn.functional.pad(x, (off, 5 - off))[:, off:off + d]
+
+    bad = h.clone()
+    if n > 1:
+        bad[n // 2] = torch.nan
+    for reduction in ("mean", "none"):
+        run_and_check(lambda a, b, r: ca.linear_cross_entropy(odd(a, 3), odd(b, 1), target, reduction=r), ref, bad, w, reduction, 64.0 if kind == "fp16" else 0.7,
+                      f"{reduction} {n} x {d}")
+        run_and_check(lambda a, b, r: ca.linear_distillation(odd(a, 2), odd(b, 3), ids, logits, temperature=2.0, reduction=r), kd, h, w, reduction,
+                      64.0 if kind == "fp16" else 0.7, f"{reduction} {n} x {d} distilled")
+
+
+def test_few_rows_one_gradient_at_a_time_and_twice():
+    h, w, target = make(40, 3000, 256, torch.bfloat16)
+    a, b, t = h.to(DEV).requires_grad_(), w.to(DEV).requires_grad_(), target.to(DEV)
+    loss = ca.linear_cross_entropy(a, b, t)
+    both = torch.autograd.grad(loss, (a, b), retain_graph=True)
+    again = torch.autograd.grad(loss, (a, b), retain_graph=True)
+    one, other = torch.autograd.grad(loss, a, retain_graph=True)[0], torch.autograd.grad(loss, b)[0]
+    frozen = torch.autograd.grad(ca.linear_cross_entropy(a, b.detach(), t), a)[0]
+    assert all(torch.equal(x, y) for x, y in zip(both + both + both[:1], again + (one, other, frozen)))
+
+
+def test_scores_that_are_not_kept_are_rebuilt():
+    """The C entries without keep_scores: the same loss, gradients within the bounds of the larger rounding."""
+    from cellseg_amd import _lib, head_losses
+    h, w, target = make(40, 3000, 256, torch.bfloat16)
+    ref = Reference(h, w, target)
+    a, b, t = h.to(DEV), w.to(DEV), target.to(DEV)
+    losses = []
+    for keep in (0, 1):
+        head = head_losses._descriptor(a, b, 0, 1, -100, 1.0, 1, t)
+        head.keep_scores = keep
+        saved = torch.empty(_lib.lib.cs_head_loss_saved_bytes(head), dtype=torch.uint8, device=DEV)
+        ws = torch.empty(max(_lib.lib.cs_head_loss_workspace_bytes(head, x) for x in (0, 3)), dtype=torch.uint8, device=DEV)
+        loss, one = torch.empty((), device=DEV), torch.ones((), device=DEV)
+        gh, gw = torch.empty_like(a), torch.empty_like(b)
+        _lib.check(_lib.lib.cs_head_loss_forward(head, None, loss.data_ptr(), saved.data_ptr(), saved.numel(), ws.data_ptr(), ws.numel(), _lib.stream_ptr()), "forward")
+        _lib.check(_lib.lib.cs_head_loss_backward(head, saved.data_ptr(), saved.numel(), one.data_ptr(), 0, gh.data_ptr(), gw.data_ptr(), ws.data_ptr(), ws.numel(),
+                                                  _lib.stream_ptr()), "backward")
+        dh, bh, dw, bw = ref.grads(torch.full((40,), 1 / 40, dtype=torch.float64))
+        within(gh, dh, bh, f"hidden, keep {keep}")
+        within(gw, dw, bw, f"weight, keep {keep}")
+        losses.append(loss)
+    assert torch.equal(*losses)
+
+
+@pytest.mark.parametrize("n,v,d", [(4200, 70001, 64), (64, 2100001, 128), (3, 700, 4098)])
+def test_a_vocabulary_of_several_pieces(n, v, d):
+    """The backward pass takes a large vocabulary in pieces (here two, the second ragged); the last case is wide instead."""
+    h, w, target = make(n, v, d, torch.bfloat16)
+    ids = torch.stack([target, (target + v // 2) % v, torch.full_like(target, v - 1)], 1)
+    logits = torch.randn(n, 3, generator=torch.Generator().manual_seed(4))
+    with torch.device(DEV):
+        ref = Reference(h.to(DEV), w.to(DEV), ids=ids.to(DEV), logits=logits.to(DEV))
+        dh, bh, dw, bw = ref.grads(torch.full((n,), 1 / n, dtype=torch.float64))
+    a, b = h.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+    loss = ca.linear_distillation(a, b, ids.to(DEV), logits.to(DEV))
+    within(loss, ref.loss.mean().cpu(), (ref.loss_bound.mean() + ref.loss.mean() * 2.0 ** -23).cpu(), "loss")
+    gh, gw = torch.autograd.grad(loss, (a, b))
+    for got, want, bound, what in ((gh, dh, bh, "hidden"), (gw, dw, bw, "weight")):
+        assert ((got.double() - want).abs() <= bound).all(), what
+
+
+def test_few_rows_captured_and_replayed_in_two_graphs():
+    h, w, target = make(20, 2000, 128, torch.bfloat16)
+    ids, logits = teacher(20, 2000, 8)
+    a, b, t = h.to(DEV).requires_grad_(), w.to(DEV).requires_grad_(), target.to(DEV)
+    ids, logits = ids.to(DEV), logits.to(DEV)
+
+    def ce():
+        loss = ca.linear_cross_entropy(a, b, t)
+        return (loss.detach(),) + torch.autograd.grad(loss, (a, b))
+
+    def kd():
+        loss = ca.linear_distillation(a, b, ids, logits, temperature=2.0)
+        return (loss.detach(),) + torch.autograd.grad(loss, (a, b))
+
+    with torch.cuda.stream(torch.cuda.Stream()):
+        ce(), kd()
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for graph, fn in zip(graphs, (ce, kd)):
+        with torch.cuda.graph(graph):
+            outs.append(fn())
+    for seed in range(3):
+        with torch.no_grad():
+            h2, w2, t2 = make(20, 2000, 128, torch.bfloat16, seed=30 + seed)
+            a.copy_(h2)
+            b.copy_(w2)
+            t.copy_(t2)
+        want = ce(), kd()
+        torch.cuda.synchronize()
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for pair in zip(want, outs) for x, y in zip(*pair))

@@ -99,3 +99,22 @@ def test_workspaces_of_no_rows():
     assert _lib.lib.cs_head_loss_saved_bytes(C.byref(h)) > 0
     for backward in range(4):
         assert _lib.lib.cs_head_loss_workspace_bytes(C.byref(h), backward) == 0
+
+
+def test_kept_scores_are_counted_and_bounded_by_the_weight():
+    """keep_scores: 64 rows at most, whole 16 rows of 128 words in fp32, and no more than the weight's own row."""
+    size = lambda **over: _lib.lib.cs_head_loss_saved_bytes(C.byref(head(hidden_pitch=512, weight_pitch=512, width=512, vocab=1000, **over)))
+    assert size(keep_scores=1) - size(keep_scores=0) == 1024 * 16 * 4
+    assert size(rows=64, keep_scores=1) - size(rows=64) == 1024 * 64 * 4
+    assert size(rows=65, keep_scores=1) == size(rows=65)
+    for rows, width, kind, kept in ((64, 128, 0, True), (64, 127, 0, False), (64, 64, 2, True), (64, 63, 2, False), (1, 32, 1, True), (1, 31, 1, False), (0, 64, 0, False)):
+        d = dict(rows=rows, width=width, type=kind, hidden_pitch=width, weight_pitch=width)
+        with_scores, without = (_lib.lib.cs_head_loss_saved_bytes(C.byref(head(keep_scores=k, **d))) for k in (1, 0))
+        assert (with_scores > without) == kept, (rows, width, kind)
+
+
+def test_sizes_beyond_a_launch_are_refused():
+    h = head(rows=1 << 24)
+    assert _lib.lib.cs_head_loss_saved_bytes(C.byref(h)) == 0
+    assert _lib.lib.cs_mxfp4_linear(4096, 8, 1, 8, 0, 4096, 4096, 1 << 28, 4096, 4096, 1 << 60, None) == -1
+    assert _lib.lib.cs_mxfp4_linear(4096, 8, 1 << 29, 8, 0, 4096, 4096, 1 << 29, 4096, 4096, 1 << 60, None) == -1

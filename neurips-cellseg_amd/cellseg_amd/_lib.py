@@ -5,6 +5,7 @@ time, and every call site raises ``CellSegHipError`` when the C side reports a f
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 
@@ -180,6 +181,21 @@ def require_gpu(tensor=None) -> None:
 def stream_ptr():
     import torch
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device):
+    """``torch.cuda.device(device)``, at no cost where it is the current one already."""
+    import torch
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def raw_stream(device) -> int:
+    """The current stream of ``device`` without a Stream object, whose making costs 17 us and more in the thread of a backward pass."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def prof_collect():

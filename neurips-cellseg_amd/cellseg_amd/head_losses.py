@@ -141,7 +141,7 @@ class _HeadLoss(torch.autograd.Function):
         top = 1 if teacher is None else ids.shape[1]
         head = _descriptor(hidden, weight, kind, reduction, ignore_index, temperature, top, ids, teacher)
         head.keep_scores = int(ctx.needs_input_grad[0] or ctx.needs_input_grad[1])
-        with torch.cuda.device(hidden.device):
+        with _lib.on_device(hidden.device):
             size = lib.cs_head_loss_saved_bytes(head)
             if not size:
                 check(-1, "cs_head_loss_saved_bytes")
@@ -150,7 +150,7 @@ class _HeadLoss(torch.autograd.Function):
             loss = torch.empty((hidden.shape[0],) if reduction == 0 else (), dtype=torch.float32, device=hidden.device)
             to = loss.data_ptr()
             check(lib.cs_head_loss_forward(head, to if reduction == 0 else None, None if reduction == 0 else to, saved.data_ptr(), saved.numel(), ws.data_ptr(), ws.numel(),
-                                           _lib.stream_ptr()), "cs_head_loss_forward")
+                                           _lib.raw_stream(hidden.device)), "cs_head_loss_forward")
         ctx.save_for_backward(hidden, weight, saved)
         ctx.head = head
         return loss
@@ -165,10 +165,10 @@ class _HeadLoss(torch.autograd.Function):
         need = ctx.needs_input_grad
         if grad.dtype != torch.float32:
             grad = grad.float()
-        with torch.cuda.device(hidden.device):
-            gh = torch.empty(hidden.shape, dtype=hidden.dtype, device=hidden.device) if need[0] else None
-            gw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device) if need[1] else None
+        with _lib.on_device(hidden.device):
+            gh = torch.empty_like(hidden, memory_format=torch.contiguous_format) if need[0] else None
+            gw = torch.empty_like(weight, memory_format=torch.contiguous_format) if need[1] else None
             ws = torch.empty(lib.cs_head_loss_workspace_bytes(head, need[0] + 2 * need[1]) or 1, dtype=torch.uint8, device=hidden.device)
             check(lib.cs_head_loss_backward(head, saved.data_ptr(), saved.numel(), grad.data_ptr(), grad.stride(0) if grad.dim() else 0, gh.data_ptr() if need[0] else None,
-                                            gw.data_ptr() if need[1] else None, ws.data_ptr(), ws.numel(), _lib.stream_ptr()), "cs_head_loss_backward")
+                                            gw.data_ptr() if need[1] else None, ws.data_ptr(), ws.numel(), _lib.raw_stream(hidden.device)), "cs_head_loss_backward")
         return gh, gw, None, None, None, None, None, None

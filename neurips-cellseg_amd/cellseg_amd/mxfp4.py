@@ -50,9 +50,9 @@ class MXFP4Tensor:
             raise TypeError(f"dtype is bfloat16, float16 or float32, got {dtype}")
         _lib.require_gpu(self.codes)
         out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        with torch.cuda.device(self.device):
+        with _lib.on_device(self.device):
             check(lib.cs_mxfp4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), out.numel() // self.width, self.width, TYPES[dtype],
-                                          out.data_ptr(), _lib.stream_ptr()), "cs_mxfp4_dequantize")
+                                          out.data_ptr(), _lib.raw_stream(self.device)), "cs_mxfp4_dequantize")
         return out
 
     def __repr__(self) -> str:
@@ -76,9 +76,9 @@ def mxfp4_quantize(x: torch.Tensor) -> MXFP4Tensor:
     blocks = -(-width // BLOCK)
     codes = torch.empty(tuple(x.shape[:-1]) + (16 * blocks,), dtype=torch.uint8, device=x.device)
     scales = torch.empty(tuple(x.shape[:-1]) + (blocks,), dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
+    with _lib.on_device(x.device):
         check(lib.cs_mxfp4_quantize(rows.data_ptr(), _pitch(rows), rows.shape[0], width, TYPES[x.dtype], codes.data_ptr(),
-                                    scales.data_ptr(), _lib.stream_ptr()), "cs_mxfp4_quantize")
+                                    scales.data_ptr(), _lib.raw_stream(x.device)), "cs_mxfp4_quantize")
     return MXFP4Tensor(codes, scales, width, x.dtype)
 
 
@@ -97,9 +97,9 @@ def mxfp4_linear(x: torch.Tensor, weight: MXFP4Tensor) -> torch.Tensor:
         raise ValueError(f"weight is on {weight.device}, x on {x.device}")
     rows, outputs = rows_of(x), weight.shape[0]
     y = torch.empty(tuple(x.shape[:-1]) + (outputs,), dtype=x.dtype, device=x.device)
-    with torch.cuda.device(x.device):
+    with _lib.on_device(x.device):
         size = lib.cs_mxfp4_linear_workspace_bytes(rows.shape[0], weight.width, outputs)
         ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
         check(lib.cs_mxfp4_linear(rows.data_ptr(), _pitch(rows), rows.shape[0], weight.width, TYPES[x.dtype], weight.codes.data_ptr(), weight.scales.data_ptr(), outputs,
-                                  y.data_ptr(), ws.data_ptr() if size else None, size, _lib.stream_ptr()), "cs_mxfp4_linear")
+                                  y.data_ptr(), ws.data_ptr() if size else None, size, _lib.raw_stream(x.device)), "cs_mxfp4_linear")
     return y

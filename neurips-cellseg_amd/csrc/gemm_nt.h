@@ -24,6 +24,10 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
+// 16 bytes at the address of any value: one instruction, as fast as an aligned one where the address is aligned
+typedef i32x4 Loose __attribute__((aligned(2)));
+typedef f32x4 LooseSum __attribute__((aligned(4)));
+
 enum Kind { BF16 = 0, FP16 = 1, FP32 = 2, E2M1 = 3 };
 
 struct Operand {
@@ -453,7 +457,7 @@ __device__ __forceinline__ void give(f32x4& sum, f32x4 v) { asm volatile("" : "=
 // A wave's tile to out[n][m] (m contiguous, `ld` elements between rows), n < rows, m < width: 16-bit rows 16 at a time, 32-bit rows 8 at a time
 // through LDS, so that a store covers whole lines (from registers it would cover runs of 32 or 64 bytes), and past the caches: written the plain
 // way the 33 MB that 256 tiles leave at once push the operands out of L2 (50176 x 4096 x 2048: 1180 TFLOP/s, with whole lines 1260, past the
-// caches 1440).  `value`: sum -> what is stored; `add`: onto what is there.  Rows that are no multiple of 16 bytes go element by element.
+// caches 1440).  `value`: sum -> what is stored; `add`: onto what is there.
 template <class T, int N> struct Stage {         // rows of N elements; chunk c of 16 bytes of row r lies at c ^ r: rows written together meet on no bank
     static constexpr int ROWS = 32 / (int)sizeof(T), LANES = N * (int)sizeof(T) / 16, BYTES = ROWS * N * (int)sizeof(T);
     static __device__ __forceinline__ int at(int row, int byte) { return (row * LANES + ((byte >> 4) ^ (row & (LANES - 1)))) * 16 + (byte & 15); }
@@ -468,7 +472,6 @@ __device__ __forceinline__ void store_tile(Tile t, char* lds, f32x4 (&acc)[R::MF
     struct alignas(16) Chunk { T v[16 / sizeof(T)]; };
     const int tid = fresh(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / R::WAVES_N, wn = wave % R::WAVES_N;
     const int m = t.m * R::TILE_M + R::row0(wm, 0) + (lane % S::LANES) * (16 / (int)sizeof(T)), g4 = (lane >> 4) * 4, col = lane & 15;
-    const bool wide = (ld * (int64_t)sizeof(T)) % 16 == 0;
     char* stage = lds + wave * S::BYTES;
 #pragma unroll
     for (int j = 0; j < R::NF; ++j)
@@ -488,13 +491,13 @@ __device__ __forceinline__ void store_tile(Tile t, char* lds, f32x4 (&acc)[R::MF
                 if (row >= S::ROWS || n >= rows || m >= width) continue;
                 Chunk c = *(const Chunk*)(stage + S::at(row, (lane % S::LANES) * 16));
                 T* to = out + (int64_t)n * ld + m;
-                if (wide) {
+                if (m + 16 / (int)sizeof(T) <= width) {
                     if (add) {
-                        const Chunk old = *(const Chunk*)to;
+                        const Chunk old = __builtin_bit_cast(Chunk, *(const Loose*)to);
 #pragma unroll
                         for (int e = 0; e < 16 / (int)sizeof(T); ++e) c.v[e] = (T)((float)c.v[e] + (float)old.v[e]);
                     }
-                    __builtin_nontemporal_store(__builtin_bit_cast(i32x4, c), (i32x4*)to);
+                    __builtin_nontemporal_store(__builtin_bit_cast(i32x4, c), (Loose*)to);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 16 / (int)sizeof(T); ++e)

@@ -694,7 +694,7 @@ __global__ __launch_bounds__(1024) void row_scale_kernel(const float* grad, int6
 // 16 bytes a lane on both sides; the tile of 8 x 8 chunks lies in LDS with chunk c of row r at c ^ (r / E), so that a column is read from all banks.
 template <class T, bool SCALED>
 __global__ __launch_bounds__(256) void transpose_kernel(const T* src, int64_t src_pitch, int64_t rows, int64_t cols, T* dst, int64_t dst_pitch, int64_t padded,
-                                                        Factors factors, bool wide) {
+                                                        Factors factors) {
     constexpr int E = 16 / (int)sizeof(T), SIDE = 8 * E, CHUNKS = SIDE * 8;
     struct alignas(16) Chunk { T v[E]; };
     __shared__ Chunk tile[CHUNKS];
@@ -706,7 +706,7 @@ __global__ __launch_bounds__(256) void transpose_kernel(const T* src, int64_t sr
         Chunk v{};
         if (row < rows && col < cols) {
             const T* from = src + row * src_pitch + col;
-            if (wide && col + E <= cols) v = *(const Chunk*)from;
+            if (col + E <= cols) v = __builtin_bit_cast(Chunk, *(const Loose*)from);
             else
 #pragma unroll
                 for (int e = 0; e < E; ++e)
@@ -732,37 +732,50 @@ __global__ __launch_bounds__(256) void transpose_kernel(const T* src, int64_t sr
     }
 }
 
-// src [rows][cols] -> dst [rows][pitch], zeros behind the columns
+// src [rows][cols] -> dst [rows][pitch] of whole 16 bytes, zeros behind the columns
 template <class T>
 __global__ __launch_bounds__(256) void copy_rows_kernel(const T* src, int64_t src_pitch, int64_t rows, int64_t cols, T* dst, int64_t pitch) {
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
-        for (int64_t c = threadIdx.x; c < pitch; c += 256) dst[r * pitch + c] = c < cols ? src[r * src_pitch + c] : (T)0.f;
+    constexpr int E = 16 / (int)sizeof(T);
+    struct alignas(16) Chunk { T v[E]; };
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)gridDim.x * 4)          // a wave takes a row
+        for (int64_t c = (threadIdx.x & 63) * E; c < pitch; c += 64 * E) {
+            const T* from = src + r * src_pitch + c;
+            Chunk v{};
+            if (c + E <= cols) v = __builtin_bit_cast(Chunk, *(const Loose*)from);
+            else
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (c + e < cols) v.v[e] = from[e];
+            *(Chunk*)(dst + r * pitch + c) = v;
+        }
 }
 
-// the sums of all runs of k, in their order, times the row's factor; 4 columns a lane where rows are multiples of 4
+// the sums of all runs of k, in their order, times the row's factor; 4 columns a lane
 template <class T>
 __global__ __launch_bounds__(256) void hidden_grad_kernel(const float* sums, int splits, int64_t rows, int64_t width, Factors factors, T* out) {
     const int64_t n = blockIdx.x, run = rows * width;
     const float f = factors.hidden(n);
     const float* from = sums + n * width;
-    if ((width & 3) == 0) {
-        struct alignas(4 * sizeof(T)) Four { T v[4]; };
-        for (int64_t c = (int64_t)threadIdx.x * 4; c < width; c += 1024) {
-            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int64_t c = (int64_t)threadIdx.x * 4; c < width; c += 1024) {
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        const int left = (int)min((int64_t)4, width - c);
+        if (left == 4) {
 #pragma unroll 8
-            for (int s = 0; s < splits; ++s) v += *(const f32x4*)(from + s * run + c);
-            Four to;
+            for (int s = 0; s < splits; ++s) v += *(const LooseSum*)(from + s * run + c);
+        } else {
+            for (int s = 0; s < splits; ++s)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) to.v[e] = (T)(f == 0.f ? 0.f : v[e] * f);
-            *(Four*)(out + n * width + c) = to;
+                for (int e = 0; e < 3; ++e)
+                    if (e < left) v[e] += from[s * run + c + e];
         }
-        return;
-    }
-    for (int64_t c = threadIdx.x; c < width; c += 256) {
-        float v = 0.f;
-#pragma unroll 8
-        for (int s = 0; s < splits; ++s) v += from[s * run + c];
-        out[n * width + c] = (T)(f == 0.f ? 0.f : v * f);
+        T to[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[e] = (T)(f == 0.f ? 0.f : v[e] * f);
+        if (left == 4) __builtin_memcpy(out + n * width + c, to, sizeof(to));
+        else
+#pragma unroll
+            for (int e = 0; e < 3; ++e)
+                if (e < left) out[n * width + c + e] = to[e];
     }
 }
 
@@ -887,9 +900,6 @@ struct Turned<FP32> {
         return sum;
     }
 };
-
-typedef i32x4 Loose __attribute__((aligned(2)));                         // 16 bytes at the address of any value
-typedef f32x4 LooseSum __attribute__((aligned(4)));
 
 struct FewGrads {
     const char *hidden, *weight;           // of the first id here
@@ -1152,14 +1162,13 @@ Plan make_plan(const cs_head_loss& h, int backward, void* base) {
 
 template <class T>
 void copy_rows(hipStream_t st, const void* src, int64_t pitch, int64_t rows, int64_t cols, void* dst, int64_t dst_pitch_bytes) {
-    copy_rows_kernel<T><<<dim3((unsigned)(rows < (1 << 20) ? rows : 1 << 20)), 256, 0, st>>>((const T*)src, pitch, rows, cols, (T*)dst, dst_pitch_bytes / (int64_t)sizeof(T));
+    copy_rows_kernel<T><<<dim3((unsigned)(rows < (1 << 22) ? (rows + 3) / 4 : 1 << 20)), 256, 0, st>>>((const T*)src, pitch, rows, cols, (T*)dst, dst_pitch_bytes / (int64_t)sizeof(T));
 }
 template <class T, bool SCALED>
 void transpose(hipStream_t st, const void* src, int64_t pitch, int64_t rows, int64_t cols, void* dst, int64_t dst_pitch, int64_t padded, const Factors& factors) {
     constexpr int SIDE = 128 / (int)sizeof(T);
-    const bool wide = ((uintptr_t)src & 15) == 0 && pitch * (int64_t)sizeof(T) % 16 == 0;
     transpose_kernel<T, SCALED><<<dim3((unsigned)((padded + SIDE - 1) / SIDE), (unsigned)((cols + SIDE - 1) / SIDE)), 256, 0, st>>>((const T*)src, pitch, rows, cols, (T*)dst,
-                                                                                                                                   dst_pitch, padded, factors, wide);
+                                                                                                                                   dst_pitch, padded, factors);
 }
 
 int check_head(const cs_head_loss* h) {

@@ -16,12 +16,14 @@ template <> struct Value<CS_TYPE_FP32> { typedef float T; };
 
 // 8 values from column c of a row of `width`
 template <class T>
-__device__ __forceinline__ void load8(const T* row, int64_t c, int64_t width, bool wide, float (&v)[8]) {
-    if (wide && c + 8 <= width) {
-        struct alignas(16) Eight { T v[8]; };
-        const Eight e = *(const Eight*)(row + c);
+__device__ __forceinline__ void load8(const T* row, int64_t c, int64_t width, float (&v)[8]) {
+    if (c + 8 <= width) {
+        struct alignas(16) Sixteen { T v[16 / sizeof(T)]; };
+        struct { Sixteen part[sizeof(T) / 2]; __device__ T at(int i) const { return part[i * sizeof(T) / 16].v[i % (16 / sizeof(T))]; } } e;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (float)e.v[i];
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) e.part[i] = __builtin_bit_cast(Sixteen, ((const Loose*)(row + c))[i]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)e.at(i);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = c + i < width ? (float)row[c + i] : 0.f;
@@ -71,12 +73,12 @@ unsigned row_blocks(int64_t rows, int64_t items) {
 }
 
 template <class T>
-__global__ __launch_bounds__(256) void quantise_kernel(const T* x, int64_t pitch, int64_t rows, int64_t width, int blocks, bool wide, uint8_t* codes, uint8_t* scales) {
+__global__ __launch_bounds__(256) void quantise_kernel(const T* x, int64_t pitch, int64_t rows, int64_t width, int blocks, uint8_t* codes, uint8_t* scales) {
     const Place p = place_of(blockIdx.x, blocks * 4);
     if (p.row >= rows) return;                                           // a block's 4 lanes go together
     for (int i = p.item; i < blocks * 4; i += 256) {
         float v[8];
-        load8(x + p.row * pitch, (int64_t)i * 8, width, wide, v);
+        load8(x + p.row * pitch, (int64_t)i * 8, width, v);
         unsigned scale;
         *(unsigned*)(codes + (p.row * blocks * 4 + i) * 4) = encode8(v, &scale);
         if ((i & 3) == 0) scales[p.row * blocks + (i >> 2)] = (uint8_t)scale;
@@ -86,7 +88,7 @@ __global__ __launch_bounds__(256) void quantise_kernel(const T* x, int64_t pitch
 // What the product reads: x quantised, and both operands' scales in its order (gemm_nt.h) over rows_x / rows_w rows, blocks up to a multiple of
 // 16, with scale 1 where there is no row or block.  The first `x_blocks` thread blocks take x, the others 64 rows of a pair of the weight's scales.
 template <class T>
-__global__ __launch_bounds__(256) void prepare_kernel(const T* x, int64_t pitch, int64_t rows, int64_t width, int blocks, bool wide, uint8_t* codes, uint8_t* scales_x,
+__global__ __launch_bounds__(256) void prepare_kernel(const T* x, int64_t pitch, int64_t rows, int64_t width, int blocks, uint8_t* codes, uint8_t* scales_x,
                                                       int64_t rows_x, const uint8_t* scales, int64_t outputs, uint8_t* scales_w, int64_t rows_w, unsigned x_blocks) {
     const int padded = (blocks + 15) / 16 * 16;
     if (blockIdx.x < x_blocks) {
@@ -95,7 +97,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(const T* x, int64_t pitch,
         for (int i = p.item; i < padded * 4; i += 256) {
             const bool in = p.row < rows && (i >> 2) < blocks;           // the same in a block's 4 lanes
             float v[8];
-            if (in) load8(x + p.row * pitch, (int64_t)i * 8, width, wide, v);
+            if (in) load8(x + p.row * pitch, (int64_t)i * 8, width, v);
             else
 #pragma unroll
                 for (int k = 0; k < 8; ++k) v[k] = 0.f;
@@ -119,7 +121,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(const T* x, int64_t pitch,
 }
 
 template <class T>
-__global__ __launch_bounds__(256) void dequantise_kernel(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t width, int blocks, bool wide, T* out) {
+__global__ __launch_bounds__(256) void dequantise_kernel(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t width, int blocks, T* out) {
     const Place p = place_of(blockIdx.x, blocks * 4);
     if (p.row >= rows) return;
     for (int i = p.item; i < blocks * 4; i += 256) {
@@ -133,9 +135,9 @@ __global__ __launch_bounds__(256) void dequantise_kernel(const uint8_t* codes, c
         for (int k = 0; k < 8; ++k) e.v[k] = (T)(v[k >> 1][k & 1] * by);
         const int64_t c = (int64_t)i * 8;
         T* to = out + p.row * width + c;
-        if (wide && c + 8 <= width) {
-            if constexpr (sizeof(T) == 2) __builtin_nontemporal_store(__builtin_bit_cast(i32x4, e), (i32x4*)to);
-            else *(Eight*)to = e;
+        if (c + 8 <= width) {
+            if constexpr (sizeof(T) == 2) __builtin_nontemporal_store(__builtin_bit_cast(i32x4, e), (Loose*)to);
+            else __builtin_memcpy(to, &e, sizeof(e));
         } else
 #pragma unroll
             for (int k = 0; k < 8; ++k)
@@ -175,7 +177,7 @@ int few_lds(int64_t rows, int64_t blocks) { return blocks > 4096 ? FEW_LDS + 1 :
 bool few_rows(int64_t rows, int64_t blocks) { return rows <= 16 && few_lds(rows, blocks) <= FEW_LDS; }
 
 template <class T>
-__global__ __launch_bounds__(256) void few_rows_kernel(const T* x, int64_t pitch, int rows, int64_t width, int blocks, bool wide, const uint8_t* codes, const uint8_t* scales,
+__global__ __launch_bounds__(256) void few_rows_kernel(const T* x, int64_t pitch, int rows, int64_t width, int blocks, const uint8_t* codes, const uint8_t* scales,
                                                        int outputs, T* y) {
     extern __shared__ __attribute__((aligned(16))) char few[];
     __shared__ f32x4 join[4][64];
@@ -201,7 +203,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const T* x, int64_t pitch
     for (int i = tid; i < rows * sp * 4; i += 256) {
         const int row = rows == 1 ? 0 : i / (sp * 4), block = (i >> 2) - row * sp;
         float v[8];
-        load8(x + row * pitch, (int64_t)block * 32 + (i & 3) * 8, width, wide, v);   // zeros behind the width
+        load8(x + row * pitch, (int64_t)block * 32 + (i & 3) * 8, width, v);   // zeros behind the width
         unsigned scale;
         *(unsigned*)(few + row * cp + block * 16 + (i & 3) * 4) = encode8(v, &scale);
         if ((i & 3) == 0) xs[row * sp + block] = (char)scale;
@@ -280,11 +282,6 @@ int check_sizes(int64_t rows, int64_t width, int type, const char* what) {
     return CS_OK;
 }
 
-template <class T>
-bool reads_wide(const void* x, int64_t pitch) {
-    return ((uintptr_t)x & 15) == 0 && (pitch * (int64_t)sizeof(T)) % 16 == 0;
-}
-
 constexpr int64_t LAUNCH_ROWS = MOST_BLOCKS / 2;       // rows of a launch, a block each at most
 
 template <class T>
@@ -292,7 +289,7 @@ int quantise(const void* x, int64_t pitch, int64_t rows, int64_t width, uint8_t*
     const int64_t blocks = (width + 31) / 32;
     for (int64_t r = 0; r < rows; r += LAUNCH_ROWS) {
         const int64_t some = rows - r < LAUNCH_ROWS ? rows - r : LAUNCH_ROWS;
-        quantise_kernel<T><<<row_blocks(some, blocks * 4), 256, 0, st>>>((const T*)x + r * pitch, pitch, some, width, (int)blocks, reads_wide<T>(x, pitch),
+        quantise_kernel<T><<<row_blocks(some, blocks * 4), 256, 0, st>>>((const T*)x + r * pitch, pitch, some, width, (int)blocks,
                                                                        codes + r * blocks * 16, scales + r * blocks);
     }
     CS_HIP(hipGetLastError());
@@ -303,7 +300,7 @@ int dequantise(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_
     const int64_t blocks = (width + 31) / 32;
     for (int64_t r = 0; r < rows; r += LAUNCH_ROWS) {
         const int64_t some = rows - r < LAUNCH_ROWS ? rows - r : LAUNCH_ROWS;
-        dequantise_kernel<T><<<row_blocks(some, blocks * 4), 256, 0, st>>>(codes + r * blocks * 16, scales + r * blocks, some, width, (int)blocks, reads_wide<T>(out, width),
+        dequantise_kernel<T><<<row_blocks(some, blocks * 4), 256, 0, st>>>(codes + r * blocks * 16, scales + r * blocks, some, width, (int)blocks,
                                                                          (T*)out + r * width);
     }
     CS_HIP(hipGetLastError());
@@ -315,14 +312,14 @@ int linear(const void* x, int64_t pitch, int64_t rows, int64_t width, const uint
     if (few_rows(rows, p.blocks)) {
         CS_REQUIRE((outputs + 15) / 16 < MOST_BLOCKS, "mxfp4 linear: too many outputs");
         few_rows_kernel<T><<<dim3((unsigned)((outputs + 15) / 16)), 256, few_lds(rows, p.blocks), st>>>((const T*)x, pitch, (int)rows, width, (int)p.blocks,
-                                                                                                   reads_wide<T>(x, pitch), codes, scales, (int)outputs, (T*)y);
+                                                                                                   codes, scales, (int)outputs, (T*)y);
         CS_HIP(hipGetLastError());
         return CS_OK;
     }
     const int64_t padded = (p.blocks + 15) / 16 * 16;
     const int64_t x_blocks = row_blocks(p.rows_x, padded * 4), w_blocks = p.rows_w / 64 * (padded / 16);
     CS_REQUIRE(x_blocks + w_blocks < MOST_BLOCKS, "mxfp4 linear: too many outputs");
-    prepare_kernel<T><<<dim3((unsigned)(x_blocks + w_blocks)), 256, 0, st>>>((const T*)x, pitch, rows, width, (int)p.blocks, reads_wide<T>(x, pitch), p.codes, p.scales_x,
+    prepare_kernel<T><<<dim3((unsigned)(x_blocks + w_blocks)), 256, 0, st>>>((const T*)x, pitch, rows, width, (int)p.blocks, p.codes, p.scales_x,
                                                                              p.rows_x, scales, outputs, p.scales_w, p.rows_w, (unsigned)x_blocks);
     CS_HIP(hipGetLastError());
     Problem q{};

@@ -361,7 +361,8 @@ int cs_dice_ce_backward(const float* logits, const int64_t* logit_strides, const
 /* ------------------------------------------------------------------------------------------------
  * Losses of a linear head over a large vocabulary (no counterpart in the reference, whose loss has 3 classes).  z = hidden weight^T is
  * never held whole: the forward pass keeps per row its maximum and sum, the backward pass rebuilds z in pieces of the vocabulary.  (Up to 64
- * rows, with keep_scores and where it takes no more than the weight, z is kept: `saved` is that much larger and the weight is read once less.)
+ * rows, with keep_scores and where it takes no more than the weight, z is kept: `saved` is that much larger and the weight is read once less.  So is z
+ * of more rows in fp32, up to 512 MB, as much as the piece of d loss / d z that the backward pass makes room for.)
  *   CS_HEAD_CROSS_ENTROPY  loss_i = lse(z_i) - z_i[target_i];  a row whose target is ignore_index has loss 0 and is not counted
  *   CS_HEAD_DISTILLATION   q_i = softmax(teacher_i / T) over the row's `top` entries, loss_i = T^2 sum_k q_ik (log q_ik - log p_i[id_ik]),
  *                          p_i = softmax(z_i / T) over the whole vocabulary.  An entry with a negative id or a teacher logit of -inf
@@ -390,7 +391,7 @@ typedef struct cs_head_loss {
     int ids_bits;               /* 32 or 64 */
     int teacher_type;           /* CS_TYPE_* */
     int top;                    /* distillation; the cross entropy takes 1 */
-    int keep_scores;            /* 1: for gradients of up to 64 rows the forward pass keeps their z, where they take no more than the weight; the same in all calls */
+    int keep_scores;            /* 1: the forward pass may keep z for the backward pass (above); the same value in all calls */
 } cs_head_loss;
 size_t cs_head_loss_saved_bytes(const cs_head_loss* head_host);
 /* backward: 0 the forward pass; else the backward pass with the gradients wanted (bit 0: hidden, bit 1: weight) */

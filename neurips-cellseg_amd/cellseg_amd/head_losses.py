@@ -1,6 +1,6 @@
 """``linear_cross_entropy`` / ``linear_distillation`` - the losses of a linear head over a large vocabulary, next to ``DiceCELoss``.
 
-The logits ``hidden @ weight.T`` are never held: the forward pass keeps the maximum and the sum of exponentials of every row, the backward
+The logits ``hidden @ weight.T`` of a large call are never held: the forward pass keeps the maximum and the sum of exponentials of every row, the backward
 pass rebuilds the logits in pieces of the vocabulary (``cs_head_loss_forward`` / ``cs_head_loss_backward``, csrc/kernels_head.hip).
 With rows i, vocabulary j, ``z = hidden weight^T``, ``p_i = softmax(z_i / T)``:
 
@@ -10,7 +10,7 @@ With rows i, vocabulary j, ``z = hidden weight^T``, ``p_i = softmax(z_i / T)``:
 ``hidden`` ``[..., D]`` and ``weight`` ``[V, D]`` share one type (bfloat16, float16 or float32) and get gradients of that type; products are
 summed, and losses returned, in float32.  16-bit gradients of the logits are rounded once to the type of the inputs before they are
 multiplied (up to 64 rows they are kept as the sum of two 16-bit values).  For gradients of up to 64 rows the logits are kept where they take
-no more memory than the weight.  A float16 net wants the usual loss scale: a mean over many rows makes gradients smaller than float16 holds.
+no more memory than the weight, and in float32, where to build them again takes longest, up to 512 MiB of them.  A float16 net wants the usual loss scale: a mean over many rows makes gradients smaller than float16 holds.
 
 Both directions can be captured into a graph; capture ``torch.autograd.grad``, as ``.backward()`` in a capture joins the stream on which an
 earlier, still living graph of the same leaves was built, which torch does not survive.

@@ -36,6 +36,8 @@ struct Saved {
     uint16_t* starts;  // [rows][starts_pitch] distillation: how many ids of the row lie below 128 t
     int64_t starts_pitch;
     float* scores;     // up to FEW_ROWS rows: z of the whole vocabulary, 1 KB a run of 32 ids and 16 rows: lane l's ids run + 4 (l / 16) + {0..3, 16..19}, row l % 16; else NULL
+    float* kept;       // fp32, more rows: z [rows][kept_pitch], or NULL
+    int64_t kept_pitch;
 };
 
 __device__ __forceinline__ int64_t id_at(const void* ids, int bits, int64_t i) {
@@ -119,6 +121,14 @@ struct NormEpi {
                     float* const to = s.scores + ((((int64_t)m0 + R::row0(wm, 0)) >> 5) * blocks + block) * 512 + lane * 8;
                     *(f32x4*)to = v[0];
                     *(f32x4*)(to + 4) = v[1];
+                }
+            }
+            if constexpr (R::KIND_ == FP32 && R::TILE_N != 32) {
+                const int n = n0 + R::col0(wn, j) + (lane & 15);
+                if (s.kept && n < rows) {
+                    float* const to = s.kept + n * s.kept_pitch + m0 + R::row0(wm, 0) + g4;
+#pragma unroll
+                    for (int i = 0; i < R::MF; ++i) *(f32x4*)(to + i * 16) = v[i];
                 }
             }
             float m = -INFINITY, sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -333,6 +343,53 @@ struct GradEpi {
         }
     }
 };
+
+// fp32: the same from a kept z.  To compute z again costs 7 times the time of its way through memory (width 768: 2 x 768 / 152 TFLOP/s against
+// 8 bytes / 5.5 TB/s for each of its values); in 16 bits no more than that, and nothing is kept there.  64 rows x 64 ids a block.
+template <bool LIST>
+__global__ __launch_bounds__(256) void kept_grad_kernel(Saved s, int rows, int vocab, int top, float c, float* g, float* gt, int64_t pitch_g, int64_t pitch_gt) {
+    __shared__ float tile[64 * 65];                                      // a column's 4 rows of 16 lanes, and 4 columns, on 64 banks
+    const int m0 = blockIdx.x * 64, n0 = blockIdx.y * 64, at = threadIdx.x & 15, m = m0 + at * 4;
+#pragma unroll
+    for (int part = 0; part < 64; part += 16) {
+        const int row = part + (threadIdx.x >> 4), n = n0 + row;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        const int state = n < rows ? s.state[n] : ROW_SKIP;
+        if (state != ROW_SKIP) {
+            const float2 norm = s.norm[n];
+            const float inv = state == ROW_BAD ? __builtin_nanf("") : norm.y;
+            const f32x4 z = *(const f32x4*)(s.kept + n * s.kept_pitch + m);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_exp2f(fmaf(z[e], c, -norm.x)) * inv;
+            if (state == ROW_COUNT) {
+                int2 listed = make_int2(0, 1);
+                if constexpr (LIST) listed = listed_of(s, n, m0 & ~127, 128);
+                for (int e = listed.x; e < listed.y; ++e) {
+                    const int64_t entry = (int64_t)n * top + e;
+                    const int want = s.ids[entry] - m;
+                    const float target = LIST ? s.q[entry] : 1.f;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) v[x] -= want == x ? target : 0.f;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = m + e < vocab ? v[e] : 0.f;
+        }
+        *(f32x4*)(g + n * pitch_g + m) = v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tile[row * 65 + at * 4 + e] = v[e];
+    }
+    if (!gt) return;
+    __syncthreads();
+#pragma unroll
+    for (int part = 0; part < 64; part += 16) {
+        const int col = part + (threadIdx.x >> 4);
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = tile[(at * 4 + e) * 65 + col];
+        *(f32x4*)(gt + (m0 + col) * pitch_gt + n0 + at * 4) = v;
+    }
+}
 
 // ---- the factor of every row.  dH of row n is hidden(n) (G W)_n; dW sums weight_row(n) h_n and is multiplied by weight().  A gradient per row is
 // divided by the largest, so that 16-bit copies of h keep their range (row_scale_kernel).  Rows that do not count get 0 by selection.
@@ -1044,6 +1101,7 @@ struct Arena {
         return p;
     }
 };
+constexpr int64_t PIECE_BYTES = (int64_t)512 << 20;      // of G
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 int type_bytes(int type) { return type == CS_TYPE_FP32 ? 4 : 2; }
 
@@ -1051,6 +1109,11 @@ int type_bytes(int type) { return type == CS_TYPE_FP32 ? 4 : 2; }
 bool few(const cs_head_loss& h) {
     const int size = type_bytes(h.type);
     return h.keep_scores && h.rows && h.rows <= FEW_ROWS && h.width * size >= 16 && up(h.rows, 16) * 4 <= h.width * size;
+}
+
+// whether the forward pass keeps z whole in fp32: where it is one piece of G, which the backward pass makes room for anyway
+bool kept(const cs_head_loss& h) {
+    return h.keep_scores && h.type == CS_TYPE_FP32 && h.rows > FEW_ROWS && up(h.rows, 256) * up(h.vocab, 256) * 4 <= PIECE_BYTES;
 }
 
 Saved carve_saved(const cs_head_loss& h, void* base, size_t* bytes) {
@@ -1068,6 +1131,8 @@ Saved carve_saved(const cs_head_loss& h, void* base, size_t* bytes) {
     s.starts = a.take<uint16_t>(kd ? n * (size_t)s.starts_pitch : 0);
     if (!kd) s.starts = nullptr;
     s.scores = few(h) ? a.take<float>((size_t)(up(h.vocab, 128) * up(h.rows, 16))) : nullptr;
+    s.kept_pitch = up(h.vocab, 256) + 32;
+    s.kept = kept(h) ? a.take<float>((size_t)(h.rows * s.kept_pitch)) : nullptr;
     *bytes = a.at;
     return s;
 }
@@ -1094,8 +1159,6 @@ struct Plan {
     int64_t runs, runs_per_split;          // few rows: of 32 ids, in a piece and for a block; blocks side by side and along the ids
     int groups, splits;
 };
-
-constexpr int64_t PIECE_BYTES = (int64_t)512 << 20;      // of G
 
 Plan make_plan(const cs_head_loss& h, int backward, void* base) {
     Plan p{};
@@ -1126,8 +1189,9 @@ Plan make_plan(const cs_head_loss& h, int backward, void* base) {
         p.bytes = a.at;
         return p;
     }
-    if (!hin) p.hidden = a.take<char>((size_t)(h.rows * width_pitch));
-    if (!win) p.weight = a.take<char>((size_t)(h.vocab * width_pitch));
+    const bool products = !backward || !kept(h);           // of hidden and weight themselves
+    if (!hin && products) p.hidden = a.take<char>((size_t)(h.rows * width_pitch));
+    if (!win && products) p.weight = a.take<char>((size_t)(h.vocab * width_pitch));
     if (!backward) {
         const Shape sh = shape_for(h.vocab, h.rows, size);
         p.part = a.take<float2>((size_t)(h.rows * ((h.vocab + SHAPES[sh].m - 1) / SHAPES[sh].m)));
@@ -1282,7 +1346,11 @@ int backward(const cs_head_loss& h, const Plan& p, const Saved& s, const float* 
         T* const g = (T*)p.g;
         T* const gt = gw ? (T*)p.gt : nullptr;
         const Shape sh = shape_for(len, h.rows, size);
-        if (int rc = kd ? launch_product<KIND>(st, sh, a, b, kbytes, whole, GradEpi<KIND, true>{g, gt, p.piece_pitch, p.row_pitch, s, (int)h.rows, (int)from, (int)len, h.top, c})
+        if (s.kept) {
+            const dim3 grid((unsigned)((len + 63) / 64), (unsigned)((h.rows + 63) / 64));
+            if (kd) kept_grad_kernel<true><<<grid, 256, 0, st>>>(s, (int)h.rows, (int)len, h.top, c, (float*)g, (float*)gt, p.piece_pitch, p.row_pitch);
+            else kept_grad_kernel<false><<<grid, 256, 0, st>>>(s, (int)h.rows, (int)len, h.top, c, (float*)g, (float*)gt, p.piece_pitch, p.row_pitch);
+        } else if (int rc = kd ? launch_product<KIND>(st, sh, a, b, kbytes, whole, GradEpi<KIND, true>{g, gt, p.piece_pitch, p.row_pitch, s, (int)h.rows, (int)from, (int)len, h.top, c})
                         : launch_product<KIND>(st, sh, a, b, kbytes, whole, GradEpi<KIND, false>{g, gt, p.piece_pitch, p.row_pitch, s, (int)h.rows, (int)from, (int)len, h.top, c}))
             return rc;
         if (gh) {

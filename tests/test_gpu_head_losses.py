@@ -416,10 +416,11 @@ def test_few_rows_one_gradient_at_a_time_and_twice():
     assert all(torch.equal(x, y) for x, y in zip(both + both + both[:1], again + (one, other, frozen)))
 
 
-def test_scores_that_are_not_kept_are_rebuilt():
+@pytest.mark.parametrize("n,v,d,kind", [(40, 3000, 256, "bf16"), (64, 1500, 96, "fp32"), (100, 1500, 77, "fp32"), (1030, 13001, 72, "fp32")])
+def test_scores_that_are_not_kept_are_rebuilt(n, v, d, kind):
     """The C entries without keep_scores: the same loss, gradients within the bounds of the larger rounding."""
     from cellseg_amd import _lib, head_losses
-    h, w, target = make(40, 3000, 256, torch.bfloat16)
+    h, w, target = make(n, v, d, TYPES[kind])
     ref = Reference(h, w, target)
     a, b, t = h.to(DEV), w.to(DEV), target.to(DEV)
     losses = []
@@ -433,7 +434,7 @@ def test_scores_that_are_not_kept_are_rebuilt():
         _lib.check(_lib.lib.cs_head_loss_forward(head, None, loss.data_ptr(), saved.data_ptr(), saved.numel(), ws.data_ptr(), ws.numel(), _lib.stream_ptr()), "forward")
         _lib.check(_lib.lib.cs_head_loss_backward(head, saved.data_ptr(), saved.numel(), one.data_ptr(), 0, gh.data_ptr(), gw.data_ptr(), ws.data_ptr(), ws.numel(),
                                                   _lib.stream_ptr()), "backward")
-        dh, bh, dw, bw = ref.grads(torch.full((40,), 1 / 40, dtype=torch.float64))
+        dh, bh, dw, bw = ref.grads(torch.full((n,), 1 / n, dtype=torch.float64))
         within(gh, dh, bh, f"hidden, keep {keep}")
         within(gw, dw, bw, f"weight, keep {keep}")
         losses.append(loss)

@@ -113,6 +113,14 @@ def test_kept_scores_are_counted_and_bounded_by_the_weight():
         assert (with_scores > without) == kept, (rows, width, kind)
 
 
+def test_kept_float32_scores_are_bounded():
+    size = lambda **over: _lib.lib.cs_head_loss_saved_bytes(C.byref(head(hidden_pitch=64, weight_pitch=64, width=64, **over)))
+    assert size(rows=100, vocab=1000, type=2, keep_scores=1) - size(rows=100, vocab=1000, type=2) == -(-100 * (1024 + 32) * 4 // 256) * 256
+    assert size(rows=100, vocab=1000, type=0, keep_scores=1) == size(rows=100, vocab=1000, type=0)
+    assert size(rows=1024, vocab=131072, type=2, keep_scores=1) > size(rows=1024, vocab=131072, type=2)
+    assert size(rows=1025, vocab=131072, type=2, keep_scores=1) == size(rows=1025, vocab=131072, type=2)
+
+
 def test_sizes_beyond_a_launch_are_refused():
     h = head(rows=1 << 24)
     assert _lib.lib.cs_head_loss_saved_bytes(C.byref(h)) == 0

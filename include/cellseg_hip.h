@@ -370,7 +370,7 @@ int cs_dice_ce_backward(const float* logits, const int64_t* logit_strides, const
  * reduction CS_REDUCE_MEAN divides the sum by the number of counted rows (no counted row: 0), in 64 bits and in a fixed order.
  * A target or id >= vocab (or a negative target other than ignore_index) makes the row's loss and gradients NaN.
  * hidden [rows][width] and weight [vocab][width] have `type`, unit inner stride and the given pitch in elements; rows whose start, pitch
- * or length is not a multiple of 16 bytes are first copied into the workspace.  Sums, maxima and losses are held in 32 bits or more.
+ * or length is not a multiple of 16 bytes may first be copied into the workspace.  Sums, maxima and losses are held in 32 bits or more.
  * The backward pass needs the same descriptor, the `saved` bytes of its forward pass, and `grad` = d / d loss (device float; for
  * CS_REDUCE_NONE one per row, grad_stride floats apart); either gradient may be NULL.  Results do not depend on the launch order (no
  * atomics).  Gradients are contiguous and start at a multiple of 16 bytes.  Limits: 1 <= width < 2^21, 1 <= vocab < 2^30, 0 <= rows < 2^24, 1 <= top <= 1024, finite temperature > 0.

@@ -246,6 +246,94 @@ struct Ring {
     }
 };
 
+// The same from rows at any address and of any length in values (k need not end with 16 bytes): through registers, two slabs ahead, since the direct
+// way into LDS wants 16-byte chunks.  For products that the bytes of A bound: a copy of A to aligned rows would cost two more passes over it.
+template <int KIND, int BM, int BN, int WM, int WN>
+struct AnyRow : Ring<KIND, BM, BN, WM, WN, 2> {
+    typedef Ring<KIND, BM, BN, WM, WN, 2> Base;
+    static constexpr int MF = Base::MF, NF = Base::NF, LOADS = Base::LOADS, STAGE_BYTES = Base::STAGE_BYTES, VALUE = KIND == FP32 ? 4 : 2;
+    static_assert(KIND != E2M1, "");
+
+    // the first `left` bytes, zeros behind them
+    static __device__ __forceinline__ i32x4 part(const char* from, int left) {
+        if (left >= 16) return *(const Loose*)from;
+        i32x4 v = {0, 0, 0, 0};
+#pragma unroll
+        for (int b = 0; b < 16; b += VALUE)
+            if (b < left) {
+                if constexpr (VALUE == 4) v[b / 4] = *(const int*)(from + b);
+                else v[b / 4] |= (int)((unsigned)*(const unsigned short*)(from + b) << (b % 4 * 8));
+            }
+        return v;
+    }
+    static __device__ __forceinline__ void run(const Problem& p, Tile t, char* lds, f32x4 (&acc)[MF][NF]) {
+        const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int wm = wave / WN, wn = wave % WN;
+        const int slabs = (p.kbytes + 127) >> 7, first = t.split * p.slabs_per_split, last = min(slabs, first + p.slabs_per_split) - 1;
+        const int64_t m0 = (int64_t)t.m * BM, n0 = (int64_t)t.n * BN;
+        const char* row_at[LOADS];
+        const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int row = (wave * LOADS + i) * 8;
+            const Operand& o = row < BM ? p.a : p.b;
+            const int64_t mine = (row < BM ? m0 + row : n0 + (row - BM)) + (lane >> 3);
+            row_at[i] = o.ptr + (mine < o.rows ? mine : o.rows - 1) * o.pitch + chunk;
+        }
+        auto fetch = [&](int slab, i32x4 (&to)[LOADS]) {
+            slab = min(slab, last);
+            const int64_t k = (int64_t)slab * 128;
+            if (k + 128 <= p.kbytes) {
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) to[i] = *(const Loose*)(row_at[i] + k);
+            } else {
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) to[i] = part(row_at[i] + k, (int)(p.kbytes - k) - chunk);
+            }
+        };
+        auto put = [&](int slot, const i32x4 (&from)[LOADS]) {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) *(i32x4*)(lds + slot * STAGE_BYTES + (wave * LOADS + i) * 1024 + lane * 16) = from[i];
+        };
+#pragma unroll
+        for (int i = 0; i < MF; ++i)
+#pragma unroll
+            for (int j = 0; j < NF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        int place[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) place[h] = (lane & 15) * 128 + (((h * 4 + (lane >> 4)) ^ (lane & 7)) * 16);
+        i32x4 x[LOADS], y[LOADS];
+        fetch(first, x);
+        fetch(first + 1, y);
+        put(0, x);
+        fetch(first + 2, x);
+        auto step = [&](int k, int slot, i32x4 (&next)[LOADS]) {
+            lds_barrier();                                               // this slab is there for every wave, and nobody reads the previous one any more
+            put(slot ^ 1, next);
+            fetch(k + 3, next);
+            const char* sa = lds + slot * STAGE_BYTES + Base::row0(wm, 0) * 128;
+            const char* sb = lds + slot * STAGE_BYTES + (BM + Base::col0(wn, 0)) * 128;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                i32x4 b[NF];
+#pragma unroll
+                for (int j = 0; j < NF; ++j) b[j] = *(const i32x4*)(sb + place[h] + j * 2048);
+#pragma unroll
+                for (int i = 0; i < MF; ++i) {
+                    const i32x4 a = *(const i32x4*)(sa + place[h] + i * 2048);
+#pragma unroll
+                    for (int j = 0; j < NF; ++j) acc[i][j] = mma<KIND, 0>(a, b[j], acc[i][j], 0, 0);
+                }
+            }
+        };
+        for (int k = first; k <= last; k += 2) {
+            step(k, 0, y);
+            if (k < last) step(k + 1, 1, x);
+        }
+        lds_barrier();                                                   // LDS is the epilogue's
+    }
+};
+
 // The large tile: 256 x 256 outputs on 4 waves of 128 x 128, one wave per SIMD.  Against 8 waves of 128 x 64 it reads 128 instead of
 // 192 KB of LDS per slab (a CU reads 128 bytes per clock and needs 2048 clocks of matrix instructions per slab), so LDS stays behind the
 // matrix pipe.  A wave multiplies a half slab (64 products, 16 clocks each) while it reads the fragments of the next:

@@ -67,6 +67,7 @@ struct NormEpi {
     Targets targets;   // cross entropy
     int rows, vocab, top;
     float c;           // log2(e) / T
+    static constexpr bool ANY_ROW = true;      // reads the caller's rows
     struct Row { int lo, hi, first, none; };
     template <class R> static constexpr int lds() { return R::TILE_N * (int)sizeof(Row) + R::WAVES_M * R::TILE_N * 8; }
     template <class R>
@@ -209,6 +210,7 @@ struct GradEpi {
     Saved s;
     int rows, from, size, top;     // this piece: ids from .. from + size
     float c;
+    static constexpr bool ANY_ROW = true;
     // fragment columns that go together: 64 rows are a line of a 16-bit G^T, and all 128 at once do not fit the registers
     template <class R> static constexpr int group() { return R::NF < 4 ? R::NF : 4; }
     template <class R> static constexpr int wave_lds() {
@@ -405,6 +407,7 @@ struct Factors {
 
 // ---- dH: fp32 sums over the pieces ------------------------------------------------------------------------------------------------
 struct SumEpi {
+    static constexpr bool ANY_ROW = false;
     float* out;        // [splits][rows][width]
     int rows, width;
     bool add;
@@ -419,6 +422,7 @@ struct SumEpi {
 // ---- dW: one rounding ---------------------------------------------------------------------------------------------------------------
 template <int KIND>
 struct OutEpi {
+    static constexpr bool ANY_ROW = false;
     typedef typename Elem<KIND>::T T;
     T* out;            // [rows of n][width]
     int rows, width;
@@ -431,6 +435,9 @@ struct OutEpi {
         store_tile<R>(t, lds, acc, out, width, rows, width, false, [f](float v) { return v * f; });
     }
 };
+
+template <int KIND> using AnyMiddle = AnyRow<KIND, 128, 128, 2, 2>;
+template <int KIND> using AnyFlat = AnyRow<KIND, 128, 32, 4, 1>;
 
 template <class R, class EPI>
 __global__ __launch_bounds__(R::THREADS) void product_kernel(Problem p, EPI epi) {
@@ -475,12 +482,17 @@ Cut cut_for(int64_t m, int64_t n, int kbytes, Shape sh, int most) {
 }
 
 template <int KIND, class EPI>
-int launch_product(hipStream_t st, Shape sh, const Operand& a, const Operand& b, int kbytes, Cut cut, const EPI& epi) {
+int launch_product(hipStream_t st, Shape sh, const Operand& a, const Operand& b, int kbytes, Cut cut, const EPI& epi, bool any_row = false) {
     Problem p{a, b, kbytes, nullptr, nullptr, 0, 0, (int)((a.rows + SHAPES[sh].m - 1) / SHAPES[sh].m), (int)((b.rows + SHAPES[sh].n - 1) / SHAPES[sh].n), cut.splits, cut.per};
     CS_REQUIRE((int64_t)p.tiles_m * p.tiles_n * p.splits < (sh == LARGE ? (int64_t)1 << 30 : MOST_BLOCKS), "head loss: too many tiles");
     if (sh == LARGE && p.kbytes % 128) product_kernel<Wide<KIND, true>, EPI><<<dim3(grid_of<Wide<KIND, true>>(p)), 256, 0, st>>>(p, epi);
     else if (sh == LARGE) product_kernel<Wide<KIND, false>, EPI><<<dim3(grid_of<Wide<KIND, false>>(p)), 256, 0, st>>>(p, epi);
-    else if (sh == MIDDLE) product_kernel<Middle<KIND>, EPI><<<dim3(grid_of<Middle<KIND>>(p)), 256, 0, st>>>(p, epi);
+    else if (any_row) {
+        if constexpr (EPI::ANY_ROW) {
+            if (sh == MIDDLE) product_kernel<AnyMiddle<KIND>, EPI><<<dim3(grid_of<AnyMiddle<KIND>>(p)), 256, 0, st>>>(p, epi);
+            else product_kernel<AnyFlat<KIND>, EPI><<<dim3(grid_of<AnyFlat<KIND>>(p)), 256, 0, st>>>(p, epi);
+        }
+    } else if (sh == MIDDLE) product_kernel<Middle<KIND>, EPI><<<dim3(grid_of<Middle<KIND>>(p)), 256, 0, st>>>(p, epi);
     else product_kernel<Flat<KIND>, EPI><<<dim3(grid_of<Flat<KIND>>(p)), 256, 0, st>>>(p, epi);
     CS_HIP(hipGetLastError());
     return CS_OK;
@@ -958,6 +970,20 @@ struct Turned<FP32> {
     }
 };
 
+// past the caches, unless rows start anywhere: their lines are then written in parts, which the caches join (4 rows, 123517 x 1311, bf16: a step
+// 341 us past the caches, 313 us through them; 65536 x 2048: 172 and 183 us)
+__device__ __forceinline__ void store_line(i32x4 v, void* to, bool aligned) {
+    if (aligned) {                                                       // the compiler would join both stores into one through the caches
+        asm volatile("; past the caches");
+        __builtin_nontemporal_store(v, (Loose*)to);
+        asm volatile("; are the whole lines");
+    } else {
+        asm volatile("; through the caches");
+        *(Loose*)to = v;
+        asm volatile("; are the parts");
+    }
+}
+
 struct FewGrads {
     const char *hidden, *weight;           // of the first id here
     int64_t hidden_pitch, weight_pitch;    // bytes, any
@@ -1051,7 +1077,7 @@ __global__ __launch_bounds__(256, BLOCKS == 1 ? 2 : 1) void few_grads_kernel(Few
 #pragma unroll
                     for (int j = 0; j < COLS; ++j) to.v[j] = (T)(dw[j][r] * f);
                     const int64_t v = run * 32 + i * 16 + q * 4 + r;
-                    if (v < p.ids) __builtin_nontemporal_store(__builtin_bit_cast(i32x4, to), (Loose*)(p.out + (v * p.width + d) * (int64_t)sizeof(T)));
+                    if (v < p.ids) store_line(__builtin_bit_cast(i32x4, to), p.out + (v * p.width + d) * (int64_t)sizeof(T), p.width * sizeof(T) % 16 == 0);
                 }
             }
     }
@@ -1145,6 +1171,7 @@ bool in_place(const void* p, int64_t pitch, int64_t width, int size) {
 struct Plan {
     size_t bytes;
     char *hidden, *weight;                 // padded copies, NULL where the tensor is read in place
+    bool any_row;                          // both are read in place whatever their alignment
     int64_t hidden_pitch, weight_pitch;    // bytes
     float2* part;
     double *losses, *entropy;
@@ -1165,7 +1192,7 @@ Plan make_plan(const cs_head_loss& h, int backward, void* base) {
     Arena a{(char*)base};
     const int size = type_bytes(h.type);
     const int64_t width_pitch = up(h.width * size, 128);
-    const bool hin = in_place(h.hidden, h.hidden_pitch, h.width, size), win = in_place(h.weight, h.weight_pitch, h.width, size);
+    bool hin = in_place(h.hidden, h.hidden_pitch, h.width, size), win = in_place(h.weight, h.weight_pitch, h.width, size);
     p.hidden_pitch = hin ? h.hidden_pitch * size : width_pitch;
     p.weight_pitch = win ? h.weight_pitch * size : width_pitch;
     if (backward && few(h)) {
@@ -1190,6 +1217,16 @@ Plan make_plan(const cs_head_loss& h, int backward, void* base) {
         return p;
     }
     const bool products = !backward || !kept(h);           // of hidden and weight themselves
+    // a weight whose rows start anywhere is read as it lies where it is read once (one column of tiles) or the products take long anyway (fp32);
+    // else it is copied (50001 x 777, bf16, the forward pass of 100 rows: 46 us against 57 copied, of 300 rows: 99 against 83)
+    int64_t some = backward && h.rows ? PIECE_BYTES / (up(h.rows, 256) * size) / 256 * 256 : h.vocab;     // words of a product
+    if (some < 256) some = 256;
+    if (some > h.vocab) some = h.vocab;
+    if (products && !win && h.rows && (h.rows <= 128 || size == 4) && shape_for(some, h.rows, size) != LARGE && h.hidden_pitch * size < (int64_t)1 << 40 && h.weight_pitch * size < (int64_t)1 << 32) {
+        p.any_row = hin = win = true;
+        p.hidden_pitch = h.hidden_pitch * size;
+        p.weight_pitch = h.weight_pitch * size;
+    }
     if (!hin && products) p.hidden = a.take<char>((size_t)(h.rows * width_pitch));
     if (!win && products) p.weight = a.take<char>((size_t)(h.vocab * width_pitch));
     if (!backward) {
@@ -1275,8 +1312,8 @@ int forward(const cs_head_loss& h, const Plan& p, const Saved& s, float* row_los
         const Shape sh = shape_for(h.vocab, h.rows, size);
         const int tiles = (int)((h.vocab + SHAPES[sh].m - 1) / SHAPES[sh].m);
         const Cut whole{1, (kbytes + 127) / 128};
-        if (int rc = kd ? launch_product<KIND>(st, sh, a, b, kbytes, whole, NormEpi<true>{p.part, s, targets, (int)h.rows, (int)h.vocab, h.top, c})
-                        : launch_product<KIND>(st, sh, a, b, kbytes, whole, NormEpi<false>{p.part, s, targets, (int)h.rows, (int)h.vocab, h.top, c}))
+        if (int rc = kd ? launch_product<KIND>(st, sh, a, b, kbytes, whole, NormEpi<true>{p.part, s, targets, (int)h.rows, (int)h.vocab, h.top, c}, p.any_row)
+                        : launch_product<KIND>(st, sh, a, b, kbytes, whole, NormEpi<false>{p.part, s, targets, (int)h.rows, (int)h.vocab, h.top, c}, p.any_row))
             return rc;
         const bool mean = h.reduction == CS_REDUCE_MEAN;
         if (h.rows <= FEW_ROWS) {
@@ -1345,13 +1382,13 @@ int backward(const cs_head_loss& h, const Plan& p, const Saved& s, const float* 
         const Cut whole{1, (kbytes + 127) / 128};
         T* const g = (T*)p.g;
         T* const gt = gw ? (T*)p.gt : nullptr;
-        const Shape sh = shape_for(len, h.rows, size);
+        const Shape sh = p.any_row && h.rows > 64 ? MIDDLE : shape_for(len, h.rows, size);
         if (s.kept) {
             const dim3 grid((unsigned)((len + 63) / 64), (unsigned)((h.rows + 63) / 64));
             if (kd) kept_grad_kernel<true><<<grid, 256, 0, st>>>(s, (int)h.rows, (int)len, h.top, c, (float*)g, (float*)gt, p.piece_pitch, p.row_pitch);
             else kept_grad_kernel<false><<<grid, 256, 0, st>>>(s, (int)h.rows, (int)len, h.top, c, (float*)g, (float*)gt, p.piece_pitch, p.row_pitch);
-        } else if (int rc = kd ? launch_product<KIND>(st, sh, a, b, kbytes, whole, GradEpi<KIND, true>{g, gt, p.piece_pitch, p.row_pitch, s, (int)h.rows, (int)from, (int)len, h.top, c})
-                        : launch_product<KIND>(st, sh, a, b, kbytes, whole, GradEpi<KIND, false>{g, gt, p.piece_pitch, p.row_pitch, s, (int)h.rows, (int)from, (int)len, h.top, c}))
+        } else if (int rc = kd ? launch_product<KIND>(st, sh, a, b, kbytes, whole, GradEpi<KIND, true>{g, gt, p.piece_pitch, p.row_pitch, s, (int)h.rows, (int)from, (int)len, h.top, c}, p.any_row)
+                        : launch_product<KIND>(st, sh, a, b, kbytes, whole, GradEpi<KIND, false>{g, gt, p.piece_pitch, p.row_pitch, s, (int)h.rows, (int)from, (int)len, h.top, c}, p.any_row))
             return rc;
         if (gh) {
             transpose<T, false>(st, (const T*)h.weight + from * h.weight_pitch, h.weight_pitch, len, h.width, p.wt, p.piece_pitch, klen, factors);

@@ -491,3 +491,17 @@ def test_few_rows_captured_and_replayed_in_two_graphs():
             graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for pair in zip(want, outs) for x, y in zip(*pair))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("n,v,d", [(100, 1500, 77), (128, 600, 333), (40, 900, 7), (129, 700, 65), (90, 300, 63)])
+def test_rows_at_any_address(n, v, d, kind):
+    """Widths that are no multiple of 16 bytes, and rows that start between them: read as they lie, or copied."""
+    h, w, target = make(n, v, d, TYPES[kind], seed=n + d)
+    target[::6] = -100
+    ids, logits = teacher(n, v, 9)
+    ref, kd = Reference(h, w, target), Reference(h, w, ids=ids, logits=logits, t=2.0)
+    ids, logits, target = ids.to(DEV), logits.to(DEV), target.to(DEV)
+    scale = 64.0 if kind == "fp16" else 0.7
+    run_and_check(lambda a, b, r: ca.linear_cross_entropy(a, torch.nn.functional.pad(b, (1, 2))[:, 1:1 + d], target, reduction=r), ref, h, w, "mean", scale, f"{n}x{v}x{d}")
+    run_and_check(lambda a, b, r: ca.linear_distillation(a, b, ids, logits, temperature=2.0, reduction=r), kd, h, w, "none", scale, f"{n}x{v}x{d} distilled")

@@ -1004,7 +1004,8 @@ struct FewGrads {
 };
 
 // A wave takes 16 bytes of 16 lanes = 256 bytes of columns and a run of ids; the four waves of a block lie side by side and share G in the caches,
-// the blocks of one run of ids lie in one XCD.  65536 x 2048, bf16, 16 rows: about 110 us for the 537 MB that are read and written (4.9 TB/s).  Behind the last column a lane computes the last whole 16 bytes again and stores the same values.
+// the blocks of one run of ids lie in one XCD.  65536 x 2048, bf16, 16 rows: about 110 us for the 537 MB that are read and written (4.9 TB/s).  Behind the last column a lane
+// computes the last whole 16 bytes again: of dW it stores the same values, of the sums of dH only the columns that no other lane has.
 template <int KIND, int BLOCKS>
 __global__ __launch_bounds__(256, BLOCKS == 1 ? 2 : 1) void few_grads_kernel(FewGrads p) {
     typedef typename Elem<KIND>::T T;
@@ -1089,6 +1090,7 @@ __global__ __launch_bounds__(256, BLOCKS == 1 ? 2 : 1) void few_grads_kernel(Few
             }
     }
     if (!p.g_h) return;
+    const int others = (chunk * 16 + col) * COLS - d;                    // how many of this lane's columns are another lane's: each is added to once
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
@@ -1099,8 +1101,14 @@ __global__ __launch_bounds__(256, BLOCKS == 1 ? 2 : 1) void few_grads_kernel(Few
 #pragma unroll
             for (int j = 0; j < COLS; j += 4) {
                 f32x4 v = {sum[b][j][r], sum[b][j + 1][r], sum[b][j + 2][r], sum[b][j + 3][r]};
-                if (p.add) v += *(const LooseSum*)(to + j);
-                *(LooseSum*)(to + j) = v;
+                if (j >= others) {
+                    if (p.add) v += *(const LooseSum*)(to + j);
+                    *(LooseSum*)(to + j) = v;
+                } else {
+#pragma unroll
+                    for (int e = 1; e < 4; ++e)
+                        if (j + e >= others) to[j + e] = p.add ? to[j + e] + v[e] : v[e];
+                }
             }
         }
 }

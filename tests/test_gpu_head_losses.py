@@ -505,3 +505,27 @@ def test_rows_at_any_address(n, v, d, kind):
     scale = 64.0 if kind == "fp16" else 0.7
     run_and_check(lambda a, b, r: ca.linear_cross_entropy(a, torch.nn.functional.pad(b, (1, 2))[:, 1:1 + d], target, reduction=r), ref, h, w, "mean", scale, f"{n}x{v}x{d}")
     run_and_check(lambda a, b, r: ca.linear_distillation(a, b, ids, logits, temperature=2.0, reduction=r), kd, h, w, "none", scale, f"{n}x{v}x{d} distilled")
+
+
+@pytest.mark.parametrize("n,d,kind", [(64, 132, "bf16"), (64, 140, "bf16"), (50, 129, "fp16"), (64, 66, "fp32")])
+def test_few_rows_over_several_pieces_add_each_column_once(n, d, kind):
+    """Widths that end inside a lane's 16 bytes, two pieces of the vocabulary: the columns that two lanes compute are added to the first piece's sums once."""
+    v, dtype = 2100001, TYPES[kind]
+    g = torch.Generator(device=DEV).manual_seed(d)
+    w = (torch.randn(v, d, generator=g, device=DEV) * 2 * d ** -0.5).to(dtype)
+    target = torch.randint(0, v, (n,), generator=g, device=DEV)
+    target[n // 2:] = v - 1 - torch.arange(n - n // 2, device=DEV)       # half of them in the last piece
+    h = (torch.randn(n, d, generator=g, device=DEV) + 1.5 * w[target].float()).to(dtype)
+    with torch.device(DEV):
+        ref = Reference(h, w, target)
+        if kind != "fp32":
+            ref.ug = unit(dtype) ** 2
+        dh, bh, dw, bw = ref.grads(torch.full((n,), 64.0 / n, dtype=torch.float64))
+    a, b = h.requires_grad_(), w.requires_grad_()
+    runs = []
+    for _ in range(2):
+        loss = ca.linear_cross_entropy(a, b, target)
+        runs.append(torch.autograd.grad(loss, (a, b), torch.tensor(64.0, device=DEV)))
+    for got, want, bound, what in zip(runs[0], (dh, dw), (bh, bw), ("hidden", "weight")):
+        assert bool(((got.double() - want).abs() <= bound).all()), what
+    assert all(torch.equal(x, y) for x, y in zip(*runs))

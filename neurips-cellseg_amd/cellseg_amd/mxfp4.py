@@ -2,13 +2,14 @@
 
 32 consecutive values of the last axis share one power-of-two scale (e8m0); each value is e2m1: 0, 0.5, 1, 1.5, 2, 3, 4 or 6 and a sign,
 4.25 bits a value in all.  ``mxfp4_linear`` rounds its input the same way and multiplies both on the 4-bit matrix instructions with float32
-sums (csrc/kernels_mxfp4.hip).  For serving: no gradients.
+sums (csrc/kernels_mxfp4.hip).  For serving: an input that wants a gradient, or carries a forward-mode tangent, is refused.
 """
 from __future__ import annotations
 
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, lib
@@ -62,6 +63,8 @@ class MXFP4Tensor:
 def _no_grad(x: torch.Tensor, name: str) -> None:
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} has no gradient: detach its input or call it under torch.no_grad()")
+    if forward_ad.unpack_dual(x).tangent is not None:
+        raise ValueError(f"{name} has no forward-mode derivative: detach its input")
 
 
 def mxfp4_quantize(x: torch.Tensor) -> MXFP4Tensor:

@@ -126,3 +126,16 @@ def test_sizes_beyond_a_launch_are_refused():
     assert _lib.lib.cs_head_loss_saved_bytes(C.byref(h)) == 0
     assert _lib.lib.cs_mxfp4_linear(4096, 8, 1, 8, 0, 4096, 4096, 1 << 28, 4096, 4096, 1 << 60, None) == -1
     assert _lib.lib.cs_mxfp4_linear(4096, 8, 1 << 29, 8, 0, 4096, 4096, 1 << 29, 4096, 4096, 1 << 60, None) == -1
+
+
+def test_a_forward_mode_tangent_is_refused():
+    """A dual tensor has requires_grad False; its result would come back without a tangent."""
+    weight = ca.MXFP4Tensor(torch.zeros(3, 16, dtype=torch.uint8), torch.zeros(3, 1, dtype=torch.uint8), 8)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(H, torch.ones_like(H))
+        for call in (lambda: ca.mxfp4_quantize(dual), lambda: ca.mxfp4_linear(dual, weight), lambda: ca.mxfp4_linear(dual[0], weight)):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="forward-mode"):
+                    call()
+        with pytest.raises(ca.CellSegHipError):                          # without its tangent it is taken, and refused for being on the CPU
+            ca.mxfp4_quantize(dual.detach())

@@ -373,7 +373,8 @@ int cs_dice_ce_backward(const float* logits, const int64_t* logit_strides, const
  * or length is not a multiple of 16 bytes may first be copied into the workspace.  Sums, maxima and losses are held in 32 bits or more.
  * The backward pass needs the same descriptor, the `saved` bytes of its forward pass, and `grad` = d / d loss (device float; for
  * CS_REDUCE_NONE one per row, grad_stride floats apart); either gradient may be NULL.  Results do not depend on the launch order (no
- * atomics).  Gradients are contiguous and start at a multiple of 16 bytes.  Limits: 1 <= width < 2^21, 1 <= vocab < 2^30, 0 <= rows < 2^24, 1 <= top <= 1024, finite temperature > 0.
+ * atomics).  Gradients are contiguous and start at a multiple of 16 bytes.  Limits: 1 <= width < 2^21, 1 <= vocab < 2^30, 0 <= rows < 2^24, 1 <= top <= 1024,
+ * 1e-5 <= temperature < 1e30, logits up to about 1e9 temperature (1e9 for the cross entropy): larger ones make the loss infinite or NaN.
  * ---------------------------------------------------------------------------------------------- */
 enum { CS_TYPE_BF16 = 0, CS_TYPE_FP16 = 1, CS_TYPE_FP32 = 2 };
 enum { CS_HEAD_CROSS_ENTROPY = 0, CS_HEAD_DISTILLATION = 1 };

@@ -29,6 +29,7 @@ TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}          # CS_TY
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}                            # CS_REDUCE_*
 _CROSS_ENTROPY, _DISTILLATION = 0, 1
 MAX_TOP = 1024
+MIN_TEMPERATURE = 1e-5
 
 
 def _pitch(t: torch.Tensor) -> int:
@@ -61,6 +62,11 @@ def _checked(hidden: torch.Tensor, weight: torch.Tensor, reduction: str, ids: to
         raise ValueError(f"hidden, weight and {name} are on one device, got {hidden.device}, {weight.device} and {ids.device}")
 
 
+def _check_temperature(temperature: float) -> None:
+    if not MIN_TEMPERATURE <= float(temperature) < 1e30:
+        raise ValueError(f"temperature is at least {MIN_TEMPERATURE:g} and finite, got {temperature}")
+
+
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *, ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
     """Softmax cross entropy of the logits ``hidden @ weight.T`` against ``target`` (``hidden.shape[:-1]``, int64 or int32) -> float32.
 
@@ -80,7 +86,9 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids:
     ``teacher_ids`` (int64 or int32) and ``teacher_logits`` (bfloat16, float16 or float32) are ``[..., K]``, K up to 1024, in any order; the
     teacher's mass is spread over them alone, the student's over the whole vocabulary.  An entry with a negative id or a logit of -inf
     carries no mass; rows without mass have loss 0, no gradient, and are not counted; an id may come twice.  An id >= V makes the loss
-    and the gradients NaN.  The teacher gets no gradient."""
+    and the gradients NaN.  The teacher gets no gradient.
+
+    ``temperature`` is 1e-5 or more: student logits beyond about 1e9 times the temperature make the loss infinite or NaN."""
     _checked(hidden, weight, reduction, teacher_ids, "teacher_ids")
     if teacher_ids.dim() != hidden.dim() or teacher_ids.shape[:-1] != hidden.shape[:-1] or teacher_logits.shape != teacher_ids.shape:
         raise ValueError(f"expected teacher_ids and teacher_logits {tuple(hidden.shape[:-1])} + (K,), got {tuple(teacher_ids.shape)} and {tuple(teacher_logits.shape)}")
@@ -92,8 +100,7 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids:
         raise ValueError(f"teacher_logits is on {teacher_logits.device}, hidden on {hidden.device}")
     if teacher_logits.requires_grad and torch.is_grad_enabled():
         raise ValueError("the teacher gets no gradient: pass teacher_logits.detach()")
-    if not 0.0 < float(temperature) < 1e30:
-        raise ValueError(f"temperature is positive and finite, got {temperature}")
+    _check_temperature(temperature)
     losses = _HeadLoss.apply(rows_of(hidden), rows_of(weight), rows_of(teacher_ids), rows_of(teacher_logits), _DISTILLATION, _REDUCTIONS[reduction], 0, float(temperature))
     return losses.reshape(hidden.shape[:-1]) if reduction == "none" else losses
 
@@ -118,8 +125,7 @@ class LinearDistillationLoss(nn.Module):
         super().__init__()
         if reduction not in _REDUCTIONS:
             raise ValueError(f"reduction is one of {', '.join(_REDUCTIONS)}, got {reduction!r}")
-        if not 0.0 < float(temperature) < 1e30:
-            raise ValueError(f"temperature is positive and finite, got {temperature}")
+        _check_temperature(temperature)
         self.temperature, self.reduction = temperature, reduction
 
     def forward(self, hidden: torch.Tensor, weight: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor) -> torch.Tensor:

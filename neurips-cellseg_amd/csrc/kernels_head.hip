@@ -19,6 +19,9 @@ using namespace nt;
 
 constexpr int KD_MAX_TOP = 1024;
 constexpr int NO_ID = 0x7fffffff;
+// c z - M is the exact c z less a float: where |c z| passes 2^31 the rounding of M alone, half its last place, leaves the range of 2^x.  From this
+// temperature on that takes logits of 14 000 and more.
+constexpr double MIN_TEMPERATURE = 1e-5;
 constexpr int FEW_ROWS = 64;
 enum RowState { ROW_SKIP = 0, ROW_COUNT = 1, ROW_BAD = 2 };
 
@@ -63,7 +66,8 @@ __device__ __forceinline__ int2 listed_of(const Saved& s, int64_t n, int from, i
 
 // ---- forward: of a tile's rows M, the largest c z rounded up, and the sum of 2^(c z - M); and the listed z ----------------------------
 // Bound by its products; the epilogue of a large tile takes 6 us of exponentials, during which the next tile's first slabs arrive (65536 words, 2048 x
-// 1024: 258 us, 1070 TFLOP/s).  M is a whole number: c z - M is one rounding from exact, and sums of different M join by exact powers of two.
+// 1024: 258 us, 1070 TFLOP/s).  M is a whole number: c z - M is one rounding from exact, and sums of different M join by exact powers of two
+// (|c z| up to 2^31: beyond 2^24 the largest lies above or below its M by half of M's last place, which 2^x still holds).
 template <bool LIST>
 struct NormEpi {
     float2* part;      // [rows][tiles_m]
@@ -1298,7 +1302,7 @@ int check_head(const cs_head_loss* h) {
     if (h->kind == CS_HEAD_DISTILLATION) {
         CS_REQUIRE(h->top >= 1 && h->top <= KD_MAX_TOP, "head loss: %d teacher logits per row: 1..%d are supported", h->top, KD_MAX_TOP);
         CS_REQUIRE(h->teacher_type >= CS_TYPE_BF16 && h->teacher_type <= CS_TYPE_FP32, "head loss: unknown teacher type %d", h->teacher_type);
-        CS_REQUIRE(h->temperature > 0.0 && h->temperature < 1e30, "head loss: temperature %g", h->temperature);
+        CS_REQUIRE(h->temperature >= MIN_TEMPERATURE && h->temperature < 1e30, "head loss: temperature %g: %g and more are supported", h->temperature, MIN_TEMPERATURE);
     } else {
         CS_REQUIRE(h->top == 1 && h->temperature == 1.0, "head loss: the cross entropy has top = 1 and temperature = 1");
     }

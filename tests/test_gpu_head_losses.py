@@ -529,3 +529,14 @@ def test_few_rows_over_several_pieces_add_each_column_once(n, d, kind):
     for got, want, bound, what in zip(runs[0], (dh, dw), (bh, bw), ("hidden", "weight")):
         assert bool(((got.double() - want).abs() <= bound).all()), what
     assert all(torch.equal(x, y) for x, y in zip(*runs))
+
+
+@pytest.mark.parametrize("n,d", [(16, 64), (100, 64)])
+def test_the_lowest_temperature_and_large_logits(n, d):
+    """Logits of several thousand at the lowest temperature, and of 1e8 at temperature 1: |z| / T up to 1e9, where a float's last place is 64."""
+    h, w, target = make(n, 500, d, torch.float32)
+    ids, logits = teacher(n, 500, 6)
+    t = 1e-5
+    run_and_check(lambda a, b, r: ca.linear_distillation(a, b, ids.to(DEV), logits.to(DEV), temperature=t, reduction=r), Reference(h * 1000, w, ids=ids, logits=logits, t=t), h * 1000, w,
+                  "mean", 1.0, "lowest temperature")
+    run_and_check(lambda a, b, r: ca.linear_cross_entropy(a, b, target.to(DEV), reduction=r), Reference(h * 2 ** 24, w, target), h * 2 ** 24, w, "none", 1.0, "large logits")

@@ -139,3 +139,17 @@ def test_a_forward_mode_tangent_is_refused():
                     call()
         with pytest.raises(ca.CellSegHipError):                          # without its tangent it is taken, and refused for being on the CPU
             ca.mxfp4_quantize(dual.detach())
+
+
+@pytest.mark.parametrize("temperature", [1e-45, 4e-39, 1e-8, 9.9e-6, float("inf")])
+def test_temperatures_that_leave_the_range_of_the_exponents_are_refused(temperature):
+    """Below 1e-8 logits of an ordinary size would come back as NaN."""
+    with pytest.raises(ValueError, match="temperature"):
+        ca.LinearDistillationLoss(temperature=temperature)
+    h = head(kind=1, teacher=4096, temperature=temperature)
+    assert _lib.lib.cs_head_loss_saved_bytes(C.byref(h)) == 0 and _lib.lib.cs_head_loss_workspace_bytes(C.byref(h), 3) == 0
+
+
+def test_the_lowest_temperature_is_taken():
+    assert ca.LinearDistillationLoss(temperature=1e-5).temperature == 1e-5
+    assert _lib.lib.cs_head_loss_saved_bytes(C.byref(head(kind=1, teacher=4096, temperature=1e-5))) > 0

@@ -62,6 +62,11 @@ def _checked(hidden: torch.Tensor, weight: torch.Tensor, reduction: str, ids: to
         raise ValueError(f"hidden, weight and {name} are on one device, got {hidden.device}, {weight.device} and {ids.device}")
 
 
+def _has_backward(hidden: torch.Tensor, weight: torch.Tensor) -> bool:
+    """Whether a backward pass can follow (``ctx.needs_input_grad`` does not know of ``torch.no_grad()``)."""
+    return torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
+
+
 def _check_temperature(temperature: float) -> None:
     if not MIN_TEMPERATURE <= float(temperature) < 1e30:
         raise ValueError(f"temperature is at least {MIN_TEMPERATURE:g} and finite, got {temperature}")
@@ -75,7 +80,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     _checked(hidden, weight, reduction, target, "target")
     if target.shape != hidden.shape[:-1]:
         raise ValueError(f"expected target {tuple(hidden.shape[:-1])}, got {tuple(target.shape)}")
-    losses = _HeadLoss.apply(rows_of(hidden), rows_of(weight), target if target.dim() == 1 else target.reshape(-1), None, _CROSS_ENTROPY, _REDUCTIONS[reduction], int(ignore_index), 1.0)
+    losses = _HeadLoss.apply(rows_of(hidden), rows_of(weight), target if target.dim() == 1 else target.reshape(-1), None, _CROSS_ENTROPY, _REDUCTIONS[reduction], int(ignore_index), 1.0,
+                             _has_backward(hidden, weight))
     return losses.reshape(target.shape) if reduction == "none" else losses
 
 
@@ -101,7 +107,8 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_ids:
     if teacher_logits.requires_grad and torch.is_grad_enabled():
         raise ValueError("the teacher gets no gradient: pass teacher_logits.detach()")
     _check_temperature(temperature)
-    losses = _HeadLoss.apply(rows_of(hidden), rows_of(weight), rows_of(teacher_ids), rows_of(teacher_logits), _DISTILLATION, _REDUCTIONS[reduction], 0, float(temperature))
+    losses = _HeadLoss.apply(rows_of(hidden), rows_of(weight), rows_of(teacher_ids), rows_of(teacher_logits), _DISTILLATION, _REDUCTIONS[reduction], 0, float(temperature),
+                             _has_backward(hidden, weight))
     return losses.reshape(hidden.shape[:-1]) if reduction == "none" else losses
 
 
@@ -143,10 +150,10 @@ def _descriptor(hidden, weight, kind, reduction, ignore_index, temperature, top,
 
 class _HeadLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, ids, teacher, kind, reduction, ignore_index, temperature):
+    def forward(ctx, hidden, weight, ids, teacher, kind, reduction, ignore_index, temperature, keep):
         top = 1 if teacher is None else ids.shape[1]
         head = _descriptor(hidden, weight, kind, reduction, ignore_index, temperature, top, ids, teacher)
-        head.keep_scores = int(ctx.needs_input_grad[0] or ctx.needs_input_grad[1])
+        head.keep_scores = int(keep)
         with _lib.on_device(hidden.device):
             size = lib.cs_head_loss_saved_bytes(head)
             if not size:
@@ -177,4 +184,4 @@ class _HeadLoss(torch.autograd.Function):
             ws = torch.empty(lib.cs_head_loss_workspace_bytes(head, need[0] + 2 * need[1]) or 1, dtype=torch.uint8, device=hidden.device)
             check(lib.cs_head_loss_backward(head, saved.data_ptr(), saved.numel(), grad.data_ptr(), grad.stride(0) if grad.dim() else 0, gh.data_ptr() if need[0] else None,
                                             gw.data_ptr() if need[1] else None, ws.data_ptr(), ws.numel(), _lib.raw_stream(hidden.device)), "cs_head_loss_backward")
-        return gh, gw, None, None, None, None, None, None
+        return gh, gw, None, None, None, None, None, None, None

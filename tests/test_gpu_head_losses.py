@@ -540,3 +540,30 @@ def test_the_lowest_temperature_and_large_logits(n, d):
     run_and_check(lambda a, b, r: ca.linear_distillation(a, b, ids.to(DEV), logits.to(DEV), temperature=t, reduction=r), Reference(h * 1000, w, ids=ids, logits=logits, t=t), h * 1000, w,
                   "mean", 1.0, "lowest temperature")
     run_and_check(lambda a, b, r: ca.linear_cross_entropy(a, b, target.to(DEV), reduction=r), Reference(h * 2 ** 24, w, target), h * 2 ** 24, w, "none", 1.0, "large logits")
+
+
+@pytest.mark.parametrize("n,d,kind", [(1000, 64, "fp32"), (64, 512, "bf16")])
+def test_no_scores_are_kept_where_no_backward_pass_can_follow(n, d, kind):
+    """Parameters under no_grad and inference_mode: the memory of detached tensors, not that of a training step."""
+    v = 16384
+    h, w, target = make(n, v, d, TYPES[kind])
+    a, b, t = h.to(DEV).requires_grad_(), w.to(DEV).requires_grad_(), target.to(DEV)
+    ids, logits = teacher(n, v, 4)
+    ids, logits = ids.to(DEV), logits.to(DEV)
+
+    def peak(a, b):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        losses = ca.linear_cross_entropy(a, b, t), ca.linear_distillation(a, b, ids, logits)
+        return torch.cuda.max_memory_allocated() - before, losses
+
+    with_scores, want = peak(a, b)
+    assert with_scores >= n * v * 4
+    alone, got = peak(a.detach(), b.detach())
+    assert all(torch.equal(x, y) for x, y in zip(want, got))
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            size, got = peak(a, b)
+        assert size == alone < n * v * 4
+        assert all(torch.equal(x, y) for x, y in zip(want, got))

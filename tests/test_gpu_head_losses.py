@@ -567,3 +567,36 @@ def test_no_scores_are_kept_where_no_backward_pass_can_follow(n, d, kind):
             size, got = peak(a, b)
         assert size == alone < n * v * 4
         assert all(torch.equal(x, y) for x, y in zip(want, got))
+
+
+@pytest.mark.parametrize("n,v,d", [(100, 1500, 64), (90, 300, 63), (1030, 13001, 72)])
+@pytest.mark.parametrize("distil", [False, True])
+@pytest.mark.parametrize("kind", ["fp16", "bf16"])
+def test_gradients_of_rows_far_apart(n, v, d, distil, kind):
+    """16 bits, a gradient per row, from 2^-24 to 1 of the largest: a word that only rows of small gradients name gets its part with all its bits.
+
+    The bound is that of one gradient for all rows: G is rounded once, to u of itself, or in fp16, where it is times its row's factor and 2^14, to 2^-25."""
+    h, w, said = make(n, v, d, TYPES[kind], seed=n, spread=8.0)         # each row is sure of one word and wrong: the words it names are its own
+    target = (said + 1 + torch.arange(n)) % v
+    ids, logits = teacher(n, v, 3)
+    size = torch.exp2(-24 * torch.rand(n, generator=torch.Generator().manual_seed(2)))
+    size[::9] = 0.0
+    size[1] = 1.0
+    per = (2048 * size).double()
+    with torch.device(DEV):
+        ref = Reference(h.to(DEV), w.to(DEV), ids=ids.to(DEV), logits=logits.to(DEV), t=2.0) if distil else Reference(h.to(DEV), w.to(DEV), target.to(DEV))
+        f = (per.to(DEV) * ref.t)[:, None]
+        g = ref.p - ref.q
+        eg = ref.p * (2 * ref.ez + 2.0 ** -16) + ref.q * 2.0 ** -23 + (ref.u + 4 * 2.0 ** -24) * g.abs()
+        dw = (f * g).t() @ ref.h
+        lost = float(f.max()) * ref.tiny * 2.0 ** -14 * (f != 0)
+        rows = (f * (eg + (n + 64) * 2.0 ** -24 * g.abs()) + lost).t() @ ref.h.abs()
+        bw = rows + ref.u * 1.01 * dw.abs() + 4 * 2.0 ** -24 * dw.abs() + ref.tiny
+    a, b = h.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+    losses = ca.linear_distillation(a, b, ids.to(DEV), logits.to(DEV), temperature=2.0, reduction="none") if distil else ca.linear_cross_entropy(a, b, target.to(DEV), reduction="none")
+    gh, gw = torch.autograd.grad(losses, (a, b), per.float().to(DEV))
+    over = ((gw.double() - dw).abs() / bw).max().item()
+    assert over <= 1, f"grad of weight: {over:.3g} of its bound"
+    dh, bh, _, _ = ref.grads(per.to(DEV))
+    assert bool(((gh.double() - dh).abs() <= bh).all())
+    assert not gh[::9].any()

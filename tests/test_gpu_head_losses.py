@@ -600,3 +600,40 @@ def test_gradients_of_rows_far_apart(n, v, d, distil, kind):
     dh, bh, _, _ = ref.grads(per.to(DEV))
     assert bool(((gh.double() - dh).abs() <= bh).all())
     assert not gh[::9].any()
+
+
+@pytest.mark.parametrize("n,v,d,kind,distil", [(1531, 32003, 1000, "fp16", False), (1550, 32003, 1000, "bf16", False), (1550, 32003, 1000, "fp16", True), (1531, 32003, 1000, "bf16", True),
+                                               (8100, 1500, 4096, "bf16", False), (1000, 16384, 2048, "fp32", False), (2050, 66001, 260, "fp32", True)])
+def test_large_tiles_one_after_the_other(n, v, d, kind, distil):
+    """More than 256 tiles of 256 x 256, of several slabs each, so that a block goes from one into the next: in the losses, in G (with and without its rows'
+    factors) and in both gradients, where k ends inside a slab and where it does not, cut and whole.  Of the 16-bit cases the first four take
+    large tiles in all four products, the fifth in the gradient of hidden with k whole; the float32 cases in the losses, and in the gradient of weight (1000
+    rows) or in G, from logits that are not kept (2050 rows)."""
+    g = torch.Generator(device=DEV).manual_seed(n + d)
+    dtype = TYPES[kind]
+    w = (torch.randn(v, d, generator=g, device=DEV) * 2 * d ** -0.5).to(dtype)
+    target = torch.randint(0, v, (n,), generator=g, device=DEV)
+    h = (torch.randn(n, d, generator=g, device=DEV) + 1.5 * w[target].float()).to(dtype)
+    with torch.device(DEV):
+        if distil:
+            ids = torch.stack([target, (target + 1) % v, (target * 7 + 5) % v, torch.full_like(target, v - 1)], 1)
+            logits = 2 * torch.randn(n, 4, generator=g)
+            ref = Reference(h, w, ids=ids, logits=logits, t=2.0)
+            per = 512 * (0.25 + torch.rand(n, generator=g))
+        else:
+            target[::7] = -100
+            ref = Reference(h, w, target)
+            per = torch.full((n,), 512.0 / int(ref.live.sum()))
+        dh, bh, dw, bw = ref.grads(per.double())
+    a, b = h.requires_grad_(), w.requires_grad_()
+    if distil:
+        loss = ca.linear_distillation(a, b, ids, logits, temperature=2.0, reduction="none")
+        assert bool(((loss.double() - ref.loss).abs() <= ref.loss_bound).all())
+    else:
+        loss = ca.linear_cross_entropy(a, b, target)
+        mean = ref.loss.sum() / ref.live.sum()
+        assert abs(loss.item() - mean.item()) <= ((ref.loss_bound.sum() / n) + mean * 2.0 ** -23).item()
+    gh, gw = torch.autograd.grad(loss, (a, b), per if distil else torch.tensor(512.0, device=DEV))
+    for got, want, bound, what in ((gh, dh, bh, "hidden"), (gw, dw, bw, "weight")):
+        over = float(((got.double() - want).abs() / bound.clamp(min=1e-300)).max())
+        assert bool(torch.isfinite(got).all()) and over <= 1, f"{what}: {over:.3g} of its bound"

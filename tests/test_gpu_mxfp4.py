@@ -194,3 +194,21 @@ def test_teacher_in_four_bits_to_a_student():
     size = float(max(weight.abs().max(), hidden.abs().max()))
     assert (a.grad.cpu().double() - c.grad).abs().max() <= (4 * ez + 2.0 ** -14) * 2 * size
     assert (b.grad.cpu().double() - e.grad).abs().max() <= (4 * ez + 2.0 ** -14) * 2 * size
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("width", [1536, 1100, 544])
+def test_linear_large_tiles_one_after_the_other(width, kind):
+    """324 tiles of 256 x 256 on 256 CUs, so that a block goes from one into the next; several pairs of slabs, that end with the width (1536) or not;
+    scales that differ by up to 2^20 from block to block, row to row and output to output."""
+    g = torch.Generator().manual_seed(width)
+    rows, outputs, blocks = 4400, 4390, -(-width // 32)
+    size = lambda n: torch.ldexp(torch.ones(n, blocks), torch.randint(-10, 10, (n, blocks), generator=g)).repeat_interleave(32, 1)[:, :width]   # noqa: E731
+    x = (torch.randn(rows, width, generator=g).clamp(-4, 4) * size(rows)).to(TYPES[kind])
+    w = torch.randn(outputs, width, generator=g) * size(outputs) / 2 ** 10
+    y = ca.mxfp4_linear(x.to(DEV), ca.mxfp4_quantize(w.to(DEV)))
+    xq, wq = definition(x)[0].to(DEV), definition(w)[0].to(DEV)
+    want = xq @ wq.t()
+    bound = (width + 8) * 2.0 ** -24 * (xq.abs() @ wq.abs().t()) + torch.finfo(x.dtype).eps / 2 * 1.01 * want.abs() + (2.0 ** -25 if kind == "fp16" else 0)
+    over = float(((y.double() - want).abs() / bound.clamp(min=1e-300)).max())
+    assert bool(torch.isfinite(y).all()) and over <= 1, f"{over:.3g} of its bound"

@@ -362,7 +362,9 @@ int cs_dice_ce_backward(const float* logits, const int64_t* logit_strides, const
  * Losses of a linear head over a large vocabulary (no counterpart in the reference, whose loss has 3 classes).  z = hidden weight^T is
  * never held whole: the forward pass keeps per row its maximum and sum, the backward pass rebuilds z in pieces of the vocabulary.  (Up to 64
  * rows, with keep_scores and where it takes no more than the weight, z is kept: `saved` is that much larger and the weight is read once less.  So is z
- * of more rows in fp32, up to 512 MB, as much as the piece of d loss / d z that the backward pass makes room for.)
+ * of more rows in fp32, up to 512 MB, as much as the piece of d loss / d z that the backward pass makes room for.)  The workspace of the backward pass
+ * is what cs_head_loss_workspace_bytes says: that piece of d loss / d z in `type` and its transpose, the piece of weight^T, fp32 sums of grad_hidden, and
+ * aligned copies; where z in fp32 would take less than about 1 GB, it is more than that.
  *   CS_HEAD_CROSS_ENTROPY  loss_i = lse(z_i) - z_i[target_i];  a row whose target is ignore_index has loss 0 and is not counted
  *   CS_HEAD_DISTILLATION   q_i = softmax(teacher_i / T) over the row's `top` entries, loss_i = T^2 sum_k q_ik (log q_ik - log p_i[id_ik]),
  *                          p_i = softmax(z_i / T) over the whole vocabulary.  An entry with a negative id or a teacher logit of -inf

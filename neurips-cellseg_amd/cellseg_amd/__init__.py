@@ -8,7 +8,7 @@ Host-side mirror of the reference's interfaces (same names, arguments and error 
   DiceCELoss / AdamW         <- monai.losses.DiceCELoss(softmax=True) / torch.optim.AdamW (baseline/model_training_3class.py:234-237)
   TrainStep                  <- the loop body baseline/model_training_3class.py:250-262 as one captured launch sequence (hipGraph)
 Beyond the reference, next to its loss and to the fp8 mode:
-  linear_cross_entropy, linear_distillation   losses of a linear head over a large vocabulary, without its logits in memory
+  linear_cross_entropy, linear_distillation   losses of a linear head over a large vocabulary, its logits in pieces
   mxfp4_quantize, mxfp4_linear                microscaled 4-bit numbers and the linear layer on them
 All arithmetic runs in libcellseg_hip.so; importing this package without the built library raises.
 """

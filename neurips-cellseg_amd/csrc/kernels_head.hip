@@ -1,4 +1,4 @@
-// gfx950 (MI355X): losses of a linear head over a large vocabulary, without its logits in memory where they are large - the cross entropy and the
+// gfx950 (MI355X): losses of a linear head over a large vocabulary, whose logits come in pieces where they are large - the cross entropy and the
 // distillation from a teacher's top logits.  Both are one computation: row i has a sparse target distribution q_i over a few ids (the
 // cross entropy: one id, q = 1) and, with u = z / T, z = H W^T, lse_i = log sum_j exp(u_ij), p = exp(u - lse):
 //   loss_i = T^2 (sum_k q_ik log q_ik + lse_i - sum_k q_ik u_i[id_ik]),   d loss_i / d z = T (p_i - q_i)
@@ -6,8 +6,8 @@
 // few z that the loss names; a wave per row joins them.  Backward, in pieces of the vocabulary: the same product again, its epilogue
 // writes G = p - q of the piece (and its transpose), then dH += G W and dW = G^T H as two products of the same kernel.  Where z is small or dear it is
 // kept instead (Saved::scores, Saved::kept).
-// Large calls are bound by the matrix pipe, at a rate that power sets: 8192 x 4096 over 131072 words, bf16: forward 6.8 ms (1290 TFLOP/s), G 7.5 ms,
-// dH and dW 6.7 ms each (1310).
+// Large calls are bound by the matrix pipe, which is busy 0.49 (G) to 0.68 (dH) of the time, at the clock that power leaves, 1.8 to 2.0 GHz.  8192 x 4096 over
+// 131072 words, bf16: forward 7.1 ms (1240 TFLOP/s), G 7.7 ms, dH and dW 6.8 ms each (1290).
 // Rows are the tokens; in every product the m axis is the one that is contiguous in what the epilogue writes (a lane holds 4 consecutive m).
 #include "gemm_nt.h"
 
@@ -190,8 +190,10 @@ struct NormEpi {
 };
 
 // ---- backward: G = p - q of a piece of the vocabulary, and its transpose ----------------------------------------------------------
-// 50000 words, 4096 x 2048: 894 us against 795 us of the same product in the forward pass.
-// The listed entries come from the z of the forward pass, p - q in fp32 before the one rounding.  Both matrices leave through LDS, 16 rows (fp32: 8)
+// 50000 words, 4096 x 2048: 929 us against 809 us of the same product in the forward pass.
+// The listed entries come from the z of the forward pass, p - q in fp32 before the one rounding.  That rounding, in 16 bits, is of the size of the gradients' own:
+// bf16, 4096 x 2048, 50000 words, each 1.66e-3 of the gradient (root mean square), both 1.92e-3 (cross entropy, whose targets' values are mostly exact) and
+// 2.33e-3 (distillation, sqrt(2) x 1.66e-3).  Two 16-bit parts, as up to 64 rows, would be 4 N V D operations on top of 8.  Both matrices leave through LDS, 16 rows (fp32: 8)
 // of a wave's tile at a time, as whole lines and past the caches: see store_tile.
 template <class T> struct alignas(4 * sizeof(T)) Four { T v[4]; };
 // 4 values rounded to T, or zeros whatever they are where `keep` is 0
@@ -377,7 +379,8 @@ struct GradEpi {
 };
 
 // fp32: the same from a kept z.  To compute z again costs 7 times the time of its way through memory (width 768: 2 x 768 / 152 TFLOP/s against
-// 8 bytes / 5.5 TB/s for each of its values); in 16 bits no more than that, and nothing is kept there.  64 rows x 64 ids a block; 1024 rows, 16384 words: 31 us for 201 MB,
+// 8 bytes / 5.5 TB/s for each of its values).  In 16 bits (1450 TFLOP/s) it costs as much as that way at a width of about 1050, 3.9 times as much at 4096; z is not
+// kept there above 64 rows, whatever the width: it would be twice the size of G, or more.  64 rows x 64 ids a block; 1024 rows, 16384 words: 31 us for 201 MB,
 // z partly from the caches, against 232 us of the product.
 template <bool LIST>
 __global__ __launch_bounds__(256) void kept_grad_kernel(Saved s, int rows, int vocab, int top, float c, float* g, float* gt, int64_t pitch_g, int64_t pitch_gt) {

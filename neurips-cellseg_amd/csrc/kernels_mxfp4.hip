@@ -4,7 +4,7 @@
 // with an infinity or NaN has the scale byte 0xff, which stands for NaN.  Two codes a byte, the even one in the low half; a row that ends
 // inside a block is filled up with zeros.
 // Quantisation and its inverse are bound by memory: 8192 x 8192, bf16, 26 and 25 us for 170 MB each (6.6 TB/s).  The product: 4096 x 4096 -> 16384
-// 132 us (4.2 PFLOP/s), its scales and x prepared in 10 us.
+// 136 us (4.0 PFLOP/s), its scales and x prepared in 10 us; both 135 to 143 us in a row of calls.
 #include "gemm_nt.h"
 
 namespace cs {
@@ -171,7 +171,7 @@ typedef Ring<E2M1, 128, 32, 4, 1, 4> Flat;
 
 // Up to 16 rows, as a server decodes: the weights are read once and nothing else counts.  A block has 16 outputs; its 4 waves take runs of 8 blocks
 // of k (128 bytes of a weight row) in turn, straight from memory into the matrix instruction, and join their sums in LDS.  Every thread block
-// quantises the few rows for itself, into LDS: one launch instead of three, and x is in L2.  1 x 4096 -> 16384: 12.6 us, 13.3 us from call to call (26.4 us in
+// quantises the few rows for itself, into LDS: one launch instead of three, and x is in L2.  1 x 4096 -> 16384: 13.1 us, 13.4 us from call to call (26.4 us in
 // three launches); 36 MB would take 6.4 us.
 constexpr int FEW_LDS = 40 << 10;                 // 4 blocks a CU
 __host__ __device__ inline int few_pitch(int blocks) { return (blocks + 3) / 4 * 64 + 16; }      // bytes of a row's codes, off the powers of two

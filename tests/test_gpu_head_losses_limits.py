@@ -184,3 +184,44 @@ def test_four_bit_tensors_of_more_than_2_to_the_31_values():
         want = xq @ wq.t()
         bound = 72 * 2.0 ** -24 * (xq.abs() @ wq.abs().t()) + 1.01 * unit(torch.bfloat16) * want.abs()
         assert bool(((y[i:i + 300].double() - want).abs() <= bound).all()), i
+
+
+@pytest.mark.parametrize("n,v,kind", [(40, 900, "bf16"), (100, 900, "fp16"), (1030, 5001, "bf16"), (100, 900, "fp32")])
+def test_a_gradient_per_row_captured_and_replayed(n, v, kind):
+    """reduction="none" in two graphs, replayed in turn with eager calls on another stream between."""
+    h, w, target = make(n, v, 128, TYPES[kind])
+    ids, logits = teacher(n, v, 5)
+    a, b, t = h.to(DEV).requires_grad_(), w.to(DEV).requires_grad_(), target.to(DEV)
+    ids, logits, per = ids.to(DEV), logits.to(DEV), torch.rand(n, device=DEV)
+
+    def ce():
+        losses = ca.linear_cross_entropy(a, b, t, reduction="none")
+        return (losses.detach(),) + torch.autograd.grad(losses, (a, b), per)
+
+    def kd():
+        losses = ca.linear_distillation(a, b, ids, logits, temperature=3.0, reduction="none")
+        return (losses.detach(),) + torch.autograd.grad(losses, (a, b), per)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        ce(), kd()
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for graph, fn in zip(graphs, (ce, kd)):
+        with torch.cuda.graph(graph):
+            outs.append(fn())
+    for seed in range(3):
+        with torch.no_grad():
+            h2, w2, t2 = make(n, v, 128, TYPES[kind], seed=40 + seed)
+            a.copy_(h2)
+            b.copy_(w2)
+            t.copy_(torch.where(torch.rand(n, generator=torch.Generator().manual_seed(seed)) < 0.2, -100, t2))
+            per.copy_(torch.exp2(-20 * torch.rand(n, generator=torch.Generator().manual_seed(seed))))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            want = ce(), kd()
+        torch.cuda.synchronize()
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for pair in zip(want, outs) for x, y in zip(*pair))
